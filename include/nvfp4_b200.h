@@ -318,6 +318,88 @@ int nvfp4_swiglu_strided(nvfp4_handle* h, const void* gate_bf16, const void* up_
 int nvfp4_swiglu_interleaved(nvfp4_handle* h, const void* gate_up_bf16, int M, int I, long long in_stride,
                              void* out_bf16, long long out_stride, nvfp4_stream_t stream);
 
+/* ---- attention over a paged cache of keys and values ---------------------
+ * What a decoder layer does between its qkv and its o linear, for a batch of sequences whose keys and values lie in
+ * pages: nvfp4_kv_append norms and rotates the new tokens' queries and keys and writes keys and values to their
+ * places, nvfp4_paged_attention reads the cache (the reference's fused qk-norm-rope, KV write, paged decode and
+ * prefill attention and its sigmoid gate: src/engine/light_ops.cu, src/engine/paged_attention.cu, layer.cu:217-404).
+ *
+ * The cache.  Token slot t of page p of head h starts at k (v) + p * page_stride + t * token_stride + h * head_stride
+ * elements, head_dim BF16 values that follow each other: [page][token][head] and [page][head][token] orders are both
+ * a matter of the strides.  head_dim 64, 128 or 256; strides are multiples of 8 elements; any page_size. */
+typedef struct nvfp4_kv_cache {
+    void* k;
+    void* v;
+    int num_pages, page_size, kv_heads, head_dim;
+    long long page_stride, token_stride, head_stride;   /* elements */
+} nvfp4_kv_cache;
+
+/* The batch.  Row r of q, k, v and out belongs to the sequence s with cu_q[s] <= r < cu_q[s+1] (cu_q NULL: one new
+ * token per sequence, row s) and stands at position kv_len[s] - (cu_q[s+1] - cu_q[s]) + (r - cu_q[s]): kv_len counts the
+ * new tokens.  Position p of sequence s lies in slot p % page_size of page block_table[s * table_stride + p / page_size].
+ * cu_q, kv_len and block_table are DEVICE memory and follow the stream like the data, so a captured call may be replayed with
+ * other contents; tokens, sequences, table_cols and max_q_len are the host's bounds and stay as captured.
+ *   tokens     rows of q, k, v and out.  Rows behind cu_q[sequences] (a padded batch) are neither read nor written.
+ *   max_q_len  the longest run of new tokens to be expected; it selects kernels, a longer run is slower, not wrong.
+ * Entries of a table row behind the sequence's last page are not used.  What the device finds out of bounds is left out, and
+ * nvfp4_device_status says so (0xA01): a page number outside [0, num_pages) or a position behind table_cols pages takes part in
+ * nothing and is not written; cu_q is clamped to [0, tokens].  Sequences may share pages that no new token lies in. */
+typedef struct nvfp4_paged_batch {
+    const int* cu_q;          /* [sequences + 1] or NULL */
+    const int* kv_len;        /* [sequences] */
+    const int* block_table;   /* [sequences, table_cols], rows table_stride entries apart */
+    long long table_stride;
+    int table_cols;
+    int sequences, tokens, max_q_len;
+} nvfp4_paged_batch;
+
+/* For each new token:  q_out = rot(norm(q, q_norm)), cache.k = rot(norm(k, k_norm)), cache.v = v, FP32 inside and one rounding.
+ *   norm   per head, x * rsqrt(mean(x^2) + norm_eps) * (1 + weight), the centred weight of nvfp4_rmsnorm; weight
+ *          [head_dim] BF16, NULL = no norm
+ *   rot    of the first rot_dim elements (a multiple of 16, 0 = none), element i with i + rot_dim / 2, by the angle
+ *          position * inv_freq[i] (inv_freq [rot_dim / 2] FP32, the product and its reduction in 64 bits, so far positions keep their
+ *          angle); positions [tokens] replaces the position as the angle's factor only (NULL: the token's own)
+ * q may be NULL with q_heads = 0.  q_out may be q itself with q's strides (in place), and overlaps nothing else.  Head and token
+ * strides in elements, multiples of 8, 0 = dense ([tokens][heads][head_dim]); k and v have the cache's heads.  All pointers on 16-byte
+ * boundaries (index arrays: 4).  A token of negative position (a padded sequence of kv_len 0) is left out; one whose place is out of
+ * bounds writes its q_out only.  Two new tokens with the same place: one of them stays, no matter which. */
+typedef struct nvfp4_kv_append_desc {
+    const nvfp4_kv_cache* cache;
+    const nvfp4_paged_batch* batch;
+    const void* q;
+    const void* k;
+    const void* v;
+    void* q_out;
+    long long q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride, q_out_stride, q_out_head_stride;
+    const void* q_norm;
+    const void* k_norm;
+    const float* inv_freq;
+    const int* positions;
+    int q_heads, rot_dim;
+    float norm_eps;
+} nvfp4_kv_append_desc;
+int nvfp4_kv_append(nvfp4_handle* h, const nvfp4_kv_append_desc* desc, nvfp4_stream_t stream);
+
+/* out[r, h] = bf16( sum_j softmax_j(scale * q[r, h] . k[j, h / g]) v[j, h / g]  (* sigmoid(gate[r, h])) ) over the positions j up to
+ * the row's own of its sequence's pages, g = q_heads / kv_heads; FP32 scores, maxima and sums, weights rounded to BF16 for the
+ * product with v.  A row that sees no key gives zeros.  scale 0 = 1 / sqrt(head_dim).  The keys and values of the new tokens must be in
+ * the cache (nvfp4_kv_append in front, on the same stream).  Slots behind a sequence's last token may hold anything, infinities and
+ * NaN included; a NaN or infinity in a value of the sequence itself reaches the rows that see it and may reach rows in front of it in
+ * the same call.  One token per sequence, a few (verification of drafted tokens), prompts and mixtures of them; work is split over the
+ * lengths found on the device and joined in a fixed order, so a result depends on the batch and its bounds, not on timing.
+ * Strides, alignment and defaults as above; out overlaps neither q, gate nor the cache.  Uses a scratch that belongs to the handle. */
+typedef struct nvfp4_paged_attention_desc {
+    const nvfp4_kv_cache* cache;
+    const nvfp4_paged_batch* batch;
+    const void* q;
+    const void* gate;
+    void* out;
+    long long q_stride, q_head_stride, gate_stride, gate_head_stride, out_stride, out_head_stride;
+    int q_heads;
+    float scale;
+} nvfp4_paged_attention_desc;
+int nvfp4_paged_attention(nvfp4_handle* h, const nvfp4_paged_attention_desc* desc, nvfp4_stream_t stream);
+
 /* ---- reference-shaped entry points --------------------------------------
  * Same argument meaning as the reference functions of the same name (void
  * return, no validation surfaced); they run on a lazily created per-device

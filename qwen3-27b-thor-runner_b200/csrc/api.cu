@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "nvfp4_internal.h"
+#include "paged_plan.h"
 
 using namespace nvfp4;
 
@@ -32,6 +33,7 @@ struct nvfp4_handle {
     int fp4_stream_min_m = 10;                   // from this token count on its activations travel through the ring (decode_fp4_stream.cu)
     int gemm_weight_rounding = 0;                // above 8 tokens: the reference's BF16-rounded weights (its GEMM branch)
     unsigned long long launches = 0;
+    char* paged_scratch = nullptr;               // parts and counters of split sequences in nvfp4_paged_attention
     int host_direct_out = 1;                     // nvfp4_linear_host: kernels store into a pinned, device-mapped C_host themselves
     // scale tensors in which nvfp4_scan_scales found a byte 0x7F / 0xFF: the tensor core reads those as NaN, so
     // these weights stay on the kernels that decode the scale themselves
@@ -294,10 +296,14 @@ int nvfp4_create(int device, size_t workspace_bytes, nvfp4_handle** out) {
     workspace_bytes &= ~(size_t)255;     // everything carved out of the workspace, from either end, stays 256-byte aligned
     e = cudaMalloc(&h->workspace, workspace_bytes);
     if (e == cudaSuccess) e = cudaMemset(h->workspace, 0, workspace_bytes);
+    const size_t paged_bytes = paged_scratch_bytes(h->dev.sm_count);
+    if (e == cudaSuccess) e = cudaMalloc(&h->paged_scratch, paged_bytes);
+    if (e == cudaSuccess) e = cudaMemset(h->paged_scratch, 0, paged_bytes);
     if (e == cudaSuccess) e = configure_kernels(h->dev);
     cudaSetDevice(prev);
     if (e != cudaSuccess) {
         if (h->workspace) cudaFree(h->workspace);
+        if (h->paged_scratch) cudaFree(h->paged_scratch);
         delete h;
         return (int)e;
     }
@@ -313,6 +319,8 @@ int nvfp4_destroy(nvfp4_handle* h) {
     cudaGetDevice(&prev);
     cudaSetDevice(h->dev.device);
     cudaError_t e = cudaFree(h->workspace);
+    const cudaError_t e2 = cudaFree(h->paged_scratch);
+    if (e == cudaSuccess) e = e2;
     cudaSetDevice(prev);
     delete h->dev.maps;
     delete h;
@@ -730,6 +738,57 @@ int nvfp4_linear_host(nvfp4_handle* h, const void* A_host, int M, const uint8_t*
         if (e != cudaSuccess) return (int)e;
     }
     return cuda_status(cudaStreamSynchronize(stream));
+}
+
+// ---- the paged cache --------------------------------------------------------------------
+
+namespace {
+
+// The calls on a paged cache run on the handle's device, whichever is current.
+struct OnDevice {
+    int prev = -1;
+    cudaError_t e = cudaSuccess;
+    explicit OnDevice(int device) {
+        int now = 0;
+        e = cudaGetDevice(&now);
+        if (e == cudaSuccess && now != device) {
+            prev = now;
+            e = cudaSetDevice(device);
+        }
+    }
+    ~OnDevice() { if (prev >= 0) cudaSetDevice(prev); }
+};
+
+}  // namespace
+
+int nvfp4_kv_append(nvfp4_handle* h, const nvfp4_kv_append_desc* d, nvfp4_stream_t stream) {
+    if (!h) return NVFP4_E_NULL;
+    paged::AppendArgs a{};
+    bool empty = false;
+    if (int e = paged::check_append(d, &a, &empty)) return e;
+    if (empty) return NVFP4_OK;
+    a.b.status = reinterpret_cast<unsigned int*>(h->workspace);
+    OnDevice on(h->dev.device);
+    if (on.e != cudaSuccess) return (int)on.e;
+    int nl = 0;
+    const cudaError_t e = launch_kv_append(a, h->dev, &nl, stream);
+    h->launches += (unsigned long long)nl;
+    return cuda_status(e);
+}
+
+int nvfp4_paged_attention(nvfp4_handle* h, const nvfp4_paged_attention_desc* d, nvfp4_stream_t stream) {
+    if (!h) return NVFP4_E_NULL;
+    paged::AttentionArgs a{};
+    bool empty = false;
+    if (int e = paged::check_attention(d, &a, &empty)) return e;
+    if (empty) return NVFP4_OK;
+    a.b.status = reinterpret_cast<unsigned int*>(h->workspace);
+    OnDevice on(h->dev.device);
+    if (on.e != cudaSuccess) return (int)on.e;
+    int nl = 0;
+    const cudaError_t e = launch_paged_decode(a, h->dev, h->paged_scratch, &nl, stream);
+    h->launches += (unsigned long long)nl;
+    return cuda_status(e);
 }
 
 // ---- reference-shaped entry points on a per-device default handle ---------------------

@@ -10,6 +10,11 @@
 
 namespace nvfp4 {
 
+namespace paged {
+struct AppendArgs;
+struct AttentionArgs;
+}  // namespace paged
+
 // Arguments of one linear call after validation.  All pointers are device pointers.
 struct LinearArgs {
     const void* A;          // [M,K] bf16
@@ -202,6 +207,13 @@ bool skinny_umma_ahead(const LinearArgs& a, const nvfp4_device_info& dev);
 cudaError_t configure_skinny_umma();
 cudaError_t launch_skinny_umma(const LinearArgs& a, nvfp4_device_info& dev, void* scratch, size_t scratch_bytes,
                                size_t offset, int* launches, cudaStream_t s);
+
+// --- the paged cache (paged_plan.h has the calls' arguments): kv_append.cu, paged_decode.cu.
+cudaError_t launch_kv_append(const paged::AppendArgs& a, const nvfp4_device_info& dev, int* launches, cudaStream_t s);
+// The attention's own scratch: joins of split sequences.  Zeroed once; every launch leaves its counters at zero.
+size_t paged_scratch_bytes(int sm_count);
+cudaError_t configure_paged_decode();
+cudaError_t launch_paged_decode(const paged::AttentionArgs& a, const nvfp4_device_info& dev, void* scratch, int* launches, cudaStream_t s);
 
 cudaError_t configure_kernels(nvfp4_device_info& dev);
 

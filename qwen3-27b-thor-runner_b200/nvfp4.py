@@ -38,6 +38,33 @@ class QuantizedWeight(ctypes.Structure):
                 ("input_scale", c_float), ("N", c_int), ("K", c_int)]
 
 
+class KvCacheStruct(ctypes.Structure):
+    """nvfp4_kv_cache of include/nvfp4_b200.h."""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("num_pages", c_int), ("page_size", c_int), ("kv_heads", c_int), ("head_dim", c_int),
+                ("page_stride", ctypes.c_longlong), ("token_stride", ctypes.c_longlong), ("head_stride", ctypes.c_longlong)]
+
+
+class PagedBatchStruct(ctypes.Structure):
+    """nvfp4_paged_batch of include/nvfp4_b200.h."""
+    _fields_ = [("cu_q", c_void_p), ("kv_len", c_void_p), ("block_table", c_void_p), ("table_stride", ctypes.c_longlong), ("table_cols", c_int),
+                ("sequences", c_int), ("tokens", c_int), ("max_q_len", c_int)]
+
+
+class KvAppendDesc(ctypes.Structure):
+    """nvfp4_kv_append_desc of include/nvfp4_b200.h."""
+    _fields_ = [(n, c_void_p) for n in ("cache", "batch", "q", "k", "v", "q_out")] + \
+               [(n, ctypes.c_longlong) for n in ("q_stride", "q_head_stride", "k_stride", "k_head_stride", "v_stride", "v_head_stride",
+                                                 "q_out_stride", "q_out_head_stride")] + \
+               [(n, c_void_p) for n in ("q_norm", "k_norm", "inv_freq", "positions")] + [("q_heads", c_int), ("rot_dim", c_int), ("norm_eps", c_float)]
+
+
+class PagedAttentionDesc(ctypes.Structure):
+    """nvfp4_paged_attention_desc of include/nvfp4_b200.h."""
+    _fields_ = [(n, c_void_p) for n in ("cache", "batch", "q", "gate", "out")] + \
+               [(n, ctypes.c_longlong) for n in ("q_stride", "q_head_stride", "gate_stride", "gate_head_stride", "out_stride", "out_head_stride")] + \
+               [("q_heads", c_int), ("scale", c_float)]
+
+
 # name -> (restype, argtypes); every symbol include/nvfp4_b200.h declares.
 SIGNATURES = {
     "nvfp4_create": (c_int, [c_int, c_size_t, ctypes.POINTER(c_void_p)]),
@@ -70,6 +97,8 @@ SIGNATURES = {
     "nvfp4_add_rmsnorm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int, c_int, c_void_p, c_void_p]),
     "nvfp4_swiglu_interleaved": (c_int, [c_void_p, c_void_p, c_int, c_int, ctypes.c_longlong, c_void_p, ctypes.c_longlong,
                                          c_void_p]),
+    "nvfp4_kv_append": (c_int, [c_void_p, c_void_p, c_void_p]),
+    "nvfp4_paged_attention": (c_int, [c_void_p, c_void_p, c_void_p]),
     "nvfp4_invoke_fp4_gemv": (None, [c_void_p, ctypes.POINTER(QuantizedWeight), c_void_p, c_void_p]),
     "nvfp4_invoke_fp4_gemv_add": (None, [c_void_p, ctypes.POINTER(QuantizedWeight), c_void_p, c_void_p,
                                          c_void_p]),
@@ -129,6 +158,45 @@ def _stream(stream):
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
+
+
+class KvCache:
+    """nvfp4_kv_cache over two BF16 tensors [pages, page size, heads, head dim] (order="token") or [pages, heads, page size, head dim]
+    (order="head") of the same strides, the last one dense."""
+
+    def __init__(self, k, v, order="token"):
+        token, head = (1, 2) if order == "token" else (2, 1)
+        if order not in ("token", "head") or k.shape != v.shape or k.stride() != v.stride() or k.dim() != 4 or k.stride(3) != 1:
+            raise ValueError("k and v: 4-D tensors of the same shape and strides, the head's values dense; order 'token' or 'head'")
+        self.keep = (k, v)
+        self.c = KvCacheStruct(k.data_ptr(), v.data_ptr(), k.shape[0], k.shape[token], k.shape[head], k.shape[3],
+                               k.stride(0), k.stride(token), k.stride(head))
+        self.address = ctypes.addressof(self.c)
+
+
+class PagedBatch:
+    """nvfp4_paged_batch: kv_len [sequences], block_table [sequences, columns] and cu_q [sequences + 1] (None: one new token per sequence)
+    are int32 device tensors whose contents may change between calls; tokens (default: one per sequence) and max_q_len are bounds."""
+
+    def __init__(self, kv_len, block_table, tokens=None, cu_q=None, max_q_len=1):
+        sequences = kv_len.shape[0]
+        for t in (kv_len, block_table, cu_q):
+            if t is not None and (t.element_size() != 4 or t.is_floating_point() or t.stride(-1) != 1):
+                raise ValueError("kv_len, block_table and cu_q are dense int32 tensors")
+        if block_table.shape[0] != sequences or (cu_q is not None and cu_q.shape[0] != sequences + 1):
+            raise ValueError("block_table has a row per sequence, cu_q an entry more than there are sequences")
+        self.keep = (kv_len, block_table, cu_q)
+        self.c = PagedBatchStruct(_ptr(cu_q), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], sequences,
+                                  sequences if tokens is None else tokens, max_q_len)
+        self.address = ctypes.addressof(self.c)
+
+
+def _rows(t):
+    """Address, token stride and head stride of a [tokens, heads, head dim] tensor."""
+    a, b, c = t.stride()
+    if c != 1 or a == 0 or b == 0:       # 0 would mean dense
+        raise ValueError("a [tokens, heads, head dim] tensor whose heads are dense and that repeats nothing")
+    return t.data_ptr(), a, b
 
 
 class Handle:
@@ -244,6 +312,25 @@ class Handle:
     def swiglu_interleaved(self, gate_up, M, I, row_stride_in, out, row_stride_out, stream=None):
         self._check(self.lib.nvfp4_swiglu_interleaved(self.h, _ptr(gate_up), M, I, row_stride_in, _ptr(out), row_stride_out,
                                                       _stream(stream)))
+
+    def kv_append(self, cache, batch, q, k, v, q_out, q_norm=None, k_norm=None, norm_eps=1e-6, inv_freq=None, positions=None, stream=None):
+        """nvfp4_kv_append: norms, rotation (of 2 * len(inv_freq) elements) and append.  q, k, v and q_out are [tokens, heads, head dim] tensors
+        (views with strides are fine; q and q_out None: keys and values only)."""
+        qp, qt, qh = (None, 0, 0) if q is None else _rows(q)
+        op, ot, oh = (None, 0, 0) if q is None else _rows(q_out)
+        kp, kt, kh = _rows(k)
+        vp, vt, vh = _rows(v)
+        d = KvAppendDesc(cache.address, batch.address, qp, kp, vp, op, qt, qh, kt, kh, vt, vh, ot, oh, _ptr(q_norm), _ptr(k_norm), _ptr(inv_freq),
+                         _ptr(positions), 0 if q is None else q.shape[1], 0 if inv_freq is None else 2 * inv_freq.shape[0], norm_eps)
+        self._check(self.lib.nvfp4_kv_append(self.h, ctypes.byref(d), _stream(stream)))
+
+    def paged_attention(self, cache, batch, q, out, gate=None, scale=0.0, stream=None):
+        """nvfp4_paged_attention: q, out and gate are [tokens, heads, head dim] tensors; scale 0 = 1 / sqrt(head dim)."""
+        qp, qt, qh = _rows(q)
+        op, ot, oh = _rows(out)
+        gp, gt, gh = (None, 0, 0) if gate is None else _rows(gate)
+        d = PagedAttentionDesc(cache.address, batch.address, qp, gp, op, qt, qh, gt, gh, ot, oh, q.shape[1], scale)
+        self._check(self.lib.nvfp4_paged_attention(self.h, ctypes.byref(d), _stream(stream)))
 
     def linear_host(self, A_host, M, packed, scale, global_scale, N, K, C_host, residual_host=None, stream=None):
         self._check(self.lib.nvfp4_linear_host(self.h, _ptr(A_host), M, _ptr(packed), _ptr(scale), global_scale,
