@@ -107,8 +107,14 @@ NVFP4_PAGED_HD bool find_row(const Batch& b, int t, int& seq, int& pos) {
 // ---- work of the attention of few tokens.  An item is a (sequence, key-value head, tile of 16 rows); it takes `chunks` units of `chunk`
 // tokens each.  All units in order (sequence, head, tile, chunk) are cut into equal runs, one per block.
 constexpr int kRows = 16;
+//
+// What an item costs beside its units (its rows of q, the warps' sums, the result's way out) is about kItemCost units, so that a run of
+// many short items would take several times as long as a run of a long one: runs are cut in places of cost, of which an item has
+// kItemCost in front of its units.  A window of more than kItemCost places holds a unit, so no run is without one.
+constexpr int kItemCost = 1;
 struct Items {
     int tiles, items, chunks;
+    NVFP4_PAGED_HD int cost() const { return chunks + kItemCost; }              // of one item
 };
 NVFP4_PAGED_HD Items items_of(const Batch& b, const Sequence& q, int group, int chunk, int most_rows) {
     Items n{0, 0, 1};
@@ -120,11 +126,39 @@ NVFP4_PAGED_HD Items items_of(const Batch& b, const Sequence& q, int group, int 
     }
     return n;
 }
-// Blocks in use: no more than there are runs of min_units.
-NVFP4_PAGED_HD int blocks_of(long long units, int grid, int min_units) { return (int)least((long long)grid, most(units / min_units, 1LL)); }
-NVFP4_PAGED_HD long long run_begin(long long units, int blocks, int block) { return units * block / blocks; }
-// The block whose run holds unit u, where no run is empty.
-NVFP4_PAGED_HD int block_of(long long units, int blocks, long long u) { return (int)(((u + 1) * blocks - 1) / units); }
+// Blocks in use: no more than there are runs of min_cost (> kItemCost) places.
+NVFP4_PAGED_HD int blocks_of(long long cost, int grid, int min_cost) { return (int)least((long long)grid, most(cost / min_cost, 1LL)); }
+NVFP4_PAGED_HD long long run_begin(long long cost, int blocks, int block) { return cost * block / blocks; }
+// The block whose run holds place c.
+NVFP4_PAGED_HD int block_of(long long cost, int blocks, long long c) { return (int)(((c + 1) * blocks - 1) / cost); }
+// The units [from, to) of an item at place `at` that lie in the run [c0, c1).
+struct Units {
+    int from, to;
+};
+NVFP4_PAGED_HD Units units_in(long long at, const Items& n, long long c0, long long c1) {
+    const long long u = at + kItemCost;
+    return {(int)least(most(c0 - u, 0LL), (long long)n.chunks), (int)least(most(c1 - u, 0LL), (long long)n.chunks)};
+}
+// The blocks that hold parts of a split item, first .. first + count - 1, count in at counters.  Up to kFlatParts parts are added by the block
+// that arrives last; more in two levels: runs of about the square root of their count by the last block of each run, then the runs' sums by the last of
+// those.  An item's first block is no other split item's first one, but its last block may be the next item's first: counters of the first
+// runs and of the second level go by `first`, those of later runs by the run's first block in a range of their own.
+constexpr int kMaxBlocks = 256, kFlatParts = 10, kMaxAdded = 16;      // kMaxAdded^2 >= kMaxBlocks: parts that one block adds at most
+constexpr int kCounters = 3 * kMaxBlocks;
+struct Join {
+    int run_len, runs;
+};
+NVFP4_PAGED_HD Join join_of(int count) {
+    Join j{count, 1};
+    if (count > kFlatParts) {
+        j.run_len = 1;
+        while (j.run_len * j.run_len < count) ++j.run_len;
+        j.runs = (count + j.run_len - 1) / j.run_len;
+    }
+    return j;
+}
+NVFP4_PAGED_HD int run_counter(int first, int run, int run_len) { return run == 0 ? first : 2 * kMaxBlocks + first + run * run_len; }
+NVFP4_PAGED_HD int item_counter(int first) { return kMaxBlocks + first; }
 
 // ---- checks of the calls' arguments
 inline bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }

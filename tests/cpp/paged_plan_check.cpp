@@ -57,31 +57,53 @@ int paged_sequence(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int s, i
     return 0;
 }
 
-// Walks the runs of all blocks over the batch's units.  0: runs are in order, none is empty, together they are all units; for every
-// item the blocks that hold a part of it are those from block_of(first unit) to block_of(last unit), and each of them has a unit of it.
-int paged_walk(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int group, int chunk, int grid, int min_units) {
+// Walks the runs of all blocks over the batch's places of cost.  0: runs are in order and together all places, each holds a unit; the units of every
+// item are shared among the blocks from that of its first unit to that of its last one, each of which has at least one, each unit once; no two counts
+// of a launch share a counter and no block adds more parts than there is room for.
+int paged_walk(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int group, int chunk, int grid, int min_cost) {
     Batch x{};
     if (check_batch(c, b, &x)) return 1;
-    long long units = 0;
-    std::vector<long long> begins;
+    long long cost = 0;
+    std::vector<long long> at;
+    std::vector<Items> items;
     for (int s = 0; s < x.sequences; ++s) {
         const Items n = items_of(x, sequence(x, s), group, chunk, 0x7fffffff);
-        for (int i = 0; i < n.items; ++i) begins.push_back(units + (long long)i * n.chunks);
-        units += (long long)n.items * n.chunks;
+        for (int i = 0; i < n.items; ++i) {
+            at.push_back(cost + (long long)i * n.cost());
+            items.push_back(n);
+        }
+        cost += (long long)n.items * n.cost();
     }
-    begins.push_back(units);
-    if (units == 0) return 0;
-    const int blocks = blocks_of(units, grid, min_units);
+    if (cost == 0) return 0;
+    const int blocks = blocks_of(cost, grid, min_cost);
     if (blocks < 1 || blocks > grid) return 2;
-    for (int k = 0; k < blocks; ++k)
-        if (run_begin(units, blocks, k) >= run_begin(units, blocks, k + 1)) return 3;
-    if (run_begin(units, blocks, 0) != 0 || run_begin(units, blocks, blocks) != units) return 4;
-    for (size_t i = 0; i + 1 < begins.size(); ++i) {
-        const int first = block_of(units, blocks, begins[i]), last = block_of(units, blocks, begins[i + 1] - 1);
-        if (first < 0 || last >= blocks || last < first) return 5;
-        if (begins[i] < run_begin(units, blocks, first) || begins[i] >= run_begin(units, blocks, first + 1)) return 6;
-        if (begins[i + 1] - 1 < run_begin(units, blocks, last) || begins[i + 1] - 1 >= run_begin(units, blocks, last + 1)) return 7;
+    if (run_begin(cost, blocks, 0) != 0 || run_begin(cost, blocks, blocks) != cost) return 3;
+    std::vector<int> used(kCounters, 0), held(blocks, 0), slots(2 * blocks, 0);
+    for (size_t i = 0; i < at.size(); ++i) {
+        const Items& n = items[i];
+        const int first = block_of(cost, blocks, at[i] + kItemCost), last = block_of(cost, blocks, at[i] + kItemCost + n.chunks - 1);
+        if (first < 0 || last >= blocks || last < first) return 4;
+        int next = 0;
+        for (int k = first > 0 ? first - 1 : 0; k <= last + 1 && k < blocks; ++k) {
+            const Units u = units_in(at[i], n, run_begin(cost, blocks, k), run_begin(cost, blocks, k + 1));
+            if ((u.from < u.to) != (k >= first && k <= last)) return 5;
+            if (u.from >= u.to) continue;
+            if (u.from != next) return 6;
+            next = u.to;
+            ++held[k];
+            if (last > first && ++slots[2 * k + (k == first)] > 1) return 7;
+        }
+        if (next != n.chunks) return 8;
+        if (last == first) continue;
+        const Join j = join_of(last - first + 1);
+        if (j.run_len < 1 || j.runs < 1 || (long long)j.run_len * j.runs < last - first + 1 || j.run_len * (j.runs - 1) >= last - first + 1) return 9;
+        if (j.run_len > kMaxAdded || j.runs > kMaxAdded) return 10;
+        for (int r = 0; r < j.runs; ++r)
+            if (++used[run_counter(first, r, j.run_len)] > 1) return 11;
+        if (j.runs > 1 && ++used[item_counter(first)] > 1) return 12;
     }
+    for (int k = 0; k < blocks; ++k)
+        if (!held[k]) return 13;
     return 0;
 }
 
