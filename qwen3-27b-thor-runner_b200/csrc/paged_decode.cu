@@ -15,11 +15,13 @@
 //  * Scores, maxima, sums and results stay in registers.  The weights 2^(t - m) are rounded to BF16 as the MMA's operand (2^-9 relative
 //    to each, below the rounding of the result); the sums take them unrounded in FP32.  The maximum follows only when a score passes it by 8
 //    (weights up to 2^8), which spares nearly every rescaling of the results.
-//  * At an item's end the warps' results are added in shared memory in warp order.  Parts of a split item go to the handle's scratch; the block
-//    that arrives last adds them in block order, so the order of arrival changes nothing.
+//  * At an item's end the warps' results are added in shared memory in warp order.  Parts of a split item go to the handle's scratch and are added
+//    in block order by a second kernel.
 // Tokens past the length, and those of pages out of bounds, are zero-filled and masked, whatever memory holds there.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "nvfp4_internal.h"
 #include "paged_plan.h"
@@ -52,16 +54,22 @@ struct Form {
     static constexpr int kRoundTiles = kTiles / kRounds;
     static constexpr int kAllTiles = D / 8, kWarpTiles = kAllTiles / kWarps;                  // tiles of the sum that a warp writes
     static constexpr int kMergeBytes = kWarps * kRoundTiles * 512;
-    static constexpr int kSmem = kWarps * kStages * kStageBytes + kMergeBytes + kWarps * kRows * 8 + kWarps * kStages * 12 + 64 + 1024;
+    static constexpr int kAhead = 16;                                  // sequences from the run's first one on that are looked up at once
+    static constexpr int kSmem = kWarps * kStages * kStageBytes + kMergeBytes + kWarps * kRows * 8 + kWarps * kStages * 12 + 64 + kAhead * 16 + 1024;
 };
 static_assert(Form<256>::kSmem <= 232448 && Form<128>::kSmem <= 232448 && Form<64>::kSmem <= 232448, "shared memory");
 static_assert(Form<256>::kStages == 3 && Form<128>::kStages == 3 && Form<64>::kStages == 6, "ring");
 static_assert(Form<256>::kMergeBytes >= 2 * Form<256>::kWarps * 1024, "the pairs' scores lie where the results are added");
 
-// Scratch of the handle: the counters, then two part slots per block: results [16 rows, D] in the layout of the registers,
-// maxima and sums.
+// Scratch of the handle: for each block the split item that begins in it, then two part slots per block: results [D / 8 tiles][32 lanes] of the
+// registers' four values, maxima and sums of the 16 rows.
+struct SplitItem {
+    int count;               // blocks that share it; 0: none begins here
+    int q0, rows, head, tile;
+    int pad[3];
+};
+constexpr size_t kSplitBytes = kMaxBlocks * sizeof(SplitItem);
 constexpr int kPartFloats = kRows * 256 + 2 * kRows;
-constexpr size_t kCounterBytes = (kCounters * 4 + 255) / 256 * 256;
 
 struct DecodeParams {
     AttentionArgs a;
@@ -69,7 +77,7 @@ struct DecodeParams {
     int min_cost;            // places of cost that a block takes at least
     int most_rows;           // sequences with more rows (new tokens x group) belong to another kernel
     int piece;               // tokens of one box of the tensor maps: 16, or 8 where pages are multiples of 8 only; 0: cp.async
-    unsigned int* counters;
+    SplitItem* split;
     float* parts;
 };
 
@@ -92,6 +100,29 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&y);
 }
 
+// Row r of an item's (token, head in the group) rows, as one lane of four sees it: two columns of every tile of eight.
+struct Row {
+    long long gate_at, out_at;
+    bool there;
+    __device__ __forceinline__ Row(const AttentionArgs& a, int q0, int rows, int head, int r) {
+        there = r < rows;
+        const int t = there ? (a.group == 1 ? r : r / a.group) : 0, h = head * a.group + (there ? r - t * a.group : 0), c = (threadIdx.x & 3) * 2;
+        gate_at = (long long)(q0 + t) * a.g_stride + (long long)h * a.g_head + c;
+        out_at = (long long)(q0 + t) * a.o_stride + (long long)h * a.o_head + c;
+    }
+    __device__ __forceinline__ uint32_t gate(const AttentionArgs& a, int tile) const {
+        return a.gate && there ? *reinterpret_cast<const uint32_t*>(a.gate + gate_at + tile * 8) : 0u;
+    }
+    // gated, rounded once
+    __device__ __forceinline__ void write(const AttentionArgs& a, int tile, uint32_t gate, float x, float y) const {
+        if (a.gate) {
+            x /= 1.0f + __expf(-__uint_as_float(gate << 16));
+            y /= 1.0f + __expf(-__uint_as_float(gate & 0xFFFF0000u));
+        }
+        if (there) *reinterpret_cast<uint32_t*>(a.out + out_at + tile * 8) = pack_bf16(x, y);
+    }
+};
+
 // A walk over the units of a run of places.
 template <int D>
 struct Cursor {
@@ -112,13 +143,14 @@ struct Cursor {
         to = u.to;
     }
     // To the next item that has units in the run [c0, c1); false behind the last one.
-    __device__ __forceinline__ bool next_item(const DecodeParams& p, long long c0, long long c1) {
+    __device__ __forceinline__ bool next_item(const DecodeParams& p, long long c0, long long c1, const Sequence* ahead, int base) {
         at += n.cost();
         if (at + kItemCost >= c1) return false;
         if (++item == n.items) {
             item = 0;
             do {
-                q = sequence(p.a.b, ++s);
+                ++s;
+                q = s - base < Form<D>::kAhead ? ahead[s - base] : sequence(p.a.b, s);
                 n = items(p, q);
             } while (n.items == 0 && s + 1 < p.a.b.sequences);
         }
@@ -143,8 +175,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     float* s_sum = s_max + F::kWarps * kRows;
     unsigned int* s_ok = reinterpret_cast<unsigned int*>(s_sum + F::kWarps * kRows);                     // [warp][stage]: tokens whose page is one
     uint64_t* full = reinterpret_cast<uint64_t*>(s_ok + F::kWarps * F::kStages) + warp * F::kStages;
-    int* s_word = reinterpret_cast<int*>(s_ok + F::kWarps * F::kStages + 2 * F::kWarps * F::kStages);
-    if (tid == 0) s_word[15] = 0;
+    int* s_abort = reinterpret_cast<int*>(s_ok + 3 * F::kWarps * F::kStages);
+    Sequence* ahead = reinterpret_cast<Sequence*>(s_abort + 16);
+    if (tid == 0) *s_abort = 0;
     if (TMA && lane == 0) {
         for (int i = 0; i < F::kStages; ++i) ptx::mbar_init(&full[i], 1);
         ptx::fence_mbar_init();
@@ -185,8 +218,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         cost += prefix[w];
     }
     upto += before;
-    if (cost == 0) return;
-    const int blocks = blocks_of(cost, gridDim.x, p.min_cost);
+    const int blocks = cost == 0 ? 0 : blocks_of(cost, gridDim.x, p.min_cost);
+    if (tid == 0) p.split[blockIdx.x].count = 0;
     if ((int)blockIdx.x >= blocks) return;
     const long long c0 = run_begin(cost, blocks, blockIdx.x), c1 = run_begin(cost, blocks, blockIdx.x + 1);
     if (upto - mine <= c0 && c0 < upto) {            // exactly one thread
@@ -206,7 +239,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     }
     __syncthreads();
     at = *found;
-    __syncthreads();                                 // the scores of pairs go to the same place
+    const int base = at.s;
+    if (tid < F::kAhead && base + tid < b.sequences) ahead[tid] = sequence(b, base + tid);
+    __syncthreads();                                 // and the scores of pairs go where the cursor was
     bool more = true;
     Cursor<D> ld = at;                               // where the loads are
     bool ld_more = more;
@@ -272,7 +307,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                     }
                 }
             }
-            if (++ld.chunk == ld.to) ld_more = ld.next_item(p, c0, c1);
+            if (++ld.chunk == ld.to) ld_more = ld.next_item(p, c0, c1, ahead, base);
             look_up();
         }
         if (!TMA) cp_async_commit();
@@ -286,44 +321,46 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     float o[F::kTiles][4];
     float m0 = 0, m1 = 0, l0 = 0, l1 = 0;            // of rows lane / 4 and lane / 4 + 8
     int see0 = 0, see1 = 0;
-    bool fresh = true;
     int stage = 0, next = F::kStages - 1;
     uint32_t parity = 0;
     unsigned int unit = 0;                           // units multiplied so far
     const int row = lane >> 2;
+    // what a new item begins with: its rows of q, and which keys they see
+    auto begin_item = [&]() {
+        const int r0 = at.tile * kRows + row, rows = at.q.q_len * a.group, head = at.head;
+        const uint16_t *x0 = nullptr, *x1 = nullptr;
+        see0 = see1 = 0x7fffffff;                    // rows that are none see all there is, of a query of zeros
+        if (r0 < rows) {
+            const int t = a.group == 1 ? r0 : r0 / a.group;
+            x0 = a.q + (long long)(at.q.q0 + t) * a.q_stride + (long long)(head * a.group + r0 - t * a.group) * a.q_head;
+            see0 = sees(at.q, t);
+        }
+        if (r0 + 8 < rows) {
+            const int t = a.group == 1 ? r0 + 8 : (r0 + 8) / a.group;
+            x1 = a.q + (long long)(at.q.q0 + t) * a.q_stride + (long long)(head * a.group + r0 + 8 - t * a.group) * a.q_head;
+            see1 = sees(at.q, t);
+        }
+#pragma unroll
+        for (int k = 0; k < F::kWidth / 16; ++k) {
+            const int c = col0 + k * 16 + (lane & 3) * 2;
+            qf[k][0] = x0 ? *reinterpret_cast<const uint32_t*>(x0 + c) : 0u;
+            qf[k][1] = x1 ? *reinterpret_cast<const uint32_t*>(x1 + c) : 0u;
+            qf[k][2] = x0 ? *reinterpret_cast<const uint32_t*>(x0 + c + 8) : 0u;
+            qf[k][3] = x1 ? *reinterpret_cast<const uint32_t*>(x1 + c + 8) : 0u;
+        }
+    };
+    auto clear = [&]() {
+#pragma unroll
+        for (int t = 0; t < F::kTiles; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
+        m0 = m1 = -INFINITY;
+        l0 = l1 = 0.0f;
+    };
+    begin_item();
+    clear();
     int from = at.chunk;                             // the first unit of the item that is this block's
     while (more) {
-        if (fresh) {                                 // a new item: its rows of q
-            fresh = false;
-            from = at.chunk;
-            const int r0 = at.tile * kRows + row, rows = at.q.q_len * a.group, head = at.head;
-            const uint16_t *x0 = nullptr, *x1 = nullptr;
-            see0 = see1 = 0x7fffffff;                // rows that are none see all there is, of a query of zeros
-            if (r0 < rows) {
-                const int t = r0 / a.group;
-                x0 = a.q + (long long)(at.q.q0 + t) * a.q_stride + (long long)(head * a.group + r0 - t * a.group) * a.q_head;
-                see0 = sees(at.q, t);
-            }
-            if (r0 + 8 < rows) {
-                const int t = (r0 + 8) / a.group;
-                x1 = a.q + (long long)(at.q.q0 + t) * a.q_stride + (long long)(head * a.group + r0 + 8 - t * a.group) * a.q_head;
-                see1 = sees(at.q, t);
-            }
-#pragma unroll
-            for (int k = 0; k < F::kWidth / 16; ++k) {
-                const int c = col0 + k * 16 + (lane & 3) * 2;
-                qf[k][0] = x0 ? *reinterpret_cast<const uint32_t*>(x0 + c) : 0u;
-                qf[k][1] = x1 ? *reinterpret_cast<const uint32_t*>(x1 + c) : 0u;
-                qf[k][2] = x0 ? *reinterpret_cast<const uint32_t*>(x0 + c + 8) : 0u;
-                qf[k][3] = x1 ? *reinterpret_cast<const uint32_t*>(x1 + c + 8) : 0u;
-            }
-#pragma unroll
-            for (int t = 0; t < F::kTiles; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
-            m0 = m1 = -INFINITY;
-            l0 = l1 = 0.0f;
-        }
         if (TMA) {
-            ptx::mbar_wait(&full[stage], parity, s_word + 15, b.status, 0xA10u);
+            ptx::mbar_wait(&full[stage], parity, s_abort, b.status, 0xA10u);
         } else {
             cp_async_wait<F::kStages - 2>();
         }
@@ -438,242 +475,342 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         if (++at.chunk < at.to) continue;
 
         // ---- the item (or this block's part of it) is through
-        fresh = true;
         const bool whole = from == 0 && at.to == at.n.chunks;
-        const int r_first = at.tile * kRows + row, rows = at.q.q_len * a.group, head = at.head;
-        // row r's place in out or gate
-        auto row_of = [&](int r, long long stride, long long head_stride) {
-            const int t = a.group == 1 ? r : r / a.group;
-            return (long long)(at.q.q0 + t) * stride + (long long)(head * a.group + r - t * a.group) * head_stride + (lane & 3) * 2;
-        };
+        const int rows = at.q.q_len * a.group, low_rows = rows - at.tile * kRows;
+        const Row row0(a, at.q.q0, rows, at.head, at.tile * kRows + row), row1(a, at.q.q0, rows, at.head, at.tile * kRows + row + 8);
+        const int first = block_of(cost, blocks, at.at + kItemCost);
+        const int count = whole ? 1 : block_of(cost, blocks, at.at + kItemCost + at.n.chunks - 1) - first + 1;
+        float* part = p.parts + (size_t)part_slot(first, blockIdx.x) * kPartFloats;
+        if (!whole && first == (int)blockIdx.x && tid == 0) p.split[blockIdx.x] = SplitItem{count, at.q.q0, rows, at.head, at.tile, {0, 0, 0}};
         // the i-th tile whose sum this warp writes: as the rounds go through them
         auto tile_of = [&](int i) {
             constexpr int kPer = F::kWarpTiles / F::kRounds;
             const int tile = i % kPer * F::kWarps + warp;
             return tile / F::kRoundTiles * F::kTiles + i / kPer * F::kRoundTiles + tile % F::kRoundTiles;
         };
-        // the gates of this thread's values, asked for in front of the barriers
-        uint32_t gates[F::kWarpTiles][2];
-        auto ask_gates = [&]() {
-            if (!a.gate) return;
-            const uint16_t* g0 = a.gate + (r_first < rows ? row_of(r_first, a.g_stride, a.g_head) : 0);
-            const uint16_t* g1 = a.gate + (r_first + 8 < rows ? row_of(r_first + 8, a.g_stride, a.g_head) : 0);
+        uint32_t gates[F::kWarpTiles][2];            // of this thread's values, asked for in front of the barriers
+        if (whole) {
 #pragma unroll
             for (int i = 0; i < F::kWarpTiles; ++i) {
-                gates[i][0] = r_first < rows ? *reinterpret_cast<const uint32_t*>(g0 + tile_of(i) * 8) : 0u;
-                gates[i][1] = r_first + 8 < rows ? *reinterpret_cast<const uint32_t*>(g1 + tile_of(i) * 8) : 0u;
+                gates[i][0] = row0.gate(a, tile_of(i));
+                gates[i][1] = row1.gate(a, tile_of(i));
             }
-        };
-        uint16_t* const out0 = a.out + (r_first < rows ? row_of(r_first, a.o_stride, a.o_head) : 0);
-        uint16_t* const out1 = a.out + (r_first + 8 < rows ? row_of(r_first + 8, a.o_stride, a.o_head) : 0);
-        // two columns of a row's result, gated, rounded once
-        auto write = [&](bool there, uint16_t* to, uint32_t gate, float x, float y) {
-            if (a.gate) {
-                x /= 1.0f + __expf(-__uint_as_float(gate << 16));
-                y /= 1.0f + __expf(-__uint_as_float(gate & 0xFFFF0000u));
-            }
-            if (there) *reinterpret_cast<uint32_t*>(to) = pack_bf16(x, y);
-        };
-        if (whole) ask_gates();
+        }
         l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
         l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
 
-        const int first = block_of(cost, blocks, at.at + kItemCost);
-        const int count = whole ? 1 : block_of(cost, blocks, at.at + kItemCost + at.n.chunks - 1) - first + 1;
-        float* part = p.parts + (size_t)(blockIdx.x * 2 + (first == (int)blockIdx.x ? 1 : 0)) * kPartFloats;
+        // the next item's rows of q are on their way while this one's results are added
+        more = at.next_item(p, c0, c1, ahead, base);
+        from = at.chunk;
+        if (more) begin_item();
         float f0[F::kGroups], f1[F::kGroups], top0 = -INFINITY, top1 = -INFINITY, sum0 = 0.0f, sum1 = 0.0f;
+        // LOW: the tile's rows are the first eight at most (a group of eight or less in decode): half the values, added in one round.
+        auto add_warps = [&](auto low) {
+            constexpr bool kLow = decltype(low)::value;
+            constexpr int kRounds = kLow ? 1 : F::kRounds, kRoundTiles = F::kTiles / kRounds, kPer = F::kWarpTiles / kRounds;
+            float2* merge2 = reinterpret_cast<float2*>(merge);
 #pragma unroll
-        for (int rd = 0; rd < F::kRounds; ++rd) {
-            __syncthreads();                         // the round before is out of the shared arrays
+            for (int rd = 0; rd < kRounds; ++rd) {
+                __syncthreads();                     // the round before is out of the shared arrays
 #pragma unroll
-            for (int i = 0; i < F::kRoundTiles; ++i) {
-                const float(&x)[4] = o[rd * F::kRoundTiles + i];
-                merge[(warp * F::kRoundTiles + i) * 32 + lane] = make_float4(x[0], x[1], x[2], x[3]);
-            }
-            if (rd == 0 && col0 == 0 && (lane & 3) == 0) {
-                s_max[group * kRows + row] = m0;
-                s_max[group * kRows + row + 8] = m1;
-                s_sum[group * kRows + row] = l0;
-                s_sum[group * kRows + row + 8] = l1;
-            }
-            __syncthreads();
-            if (rd == 0) {
-#pragma unroll
-                for (int w = 0; w < F::kGroups; ++w) {
-                    f0[w] = s_max[w * kRows + row];
-                    f1[w] = s_max[w * kRows + row + 8];
-                    top0 = fmaxf(top0, f0[w]);
-                    top1 = fmaxf(top1, f1[w]);
+                for (int i = 0; i < kRoundTiles; ++i) {
+                    const float(&x)[4] = o[rd * kRoundTiles + i];
+                    if (kLow) merge2[(warp * kRoundTiles + i) * 32 + lane] = make_float2(x[0], x[1]);
+                    else merge[(warp * kRoundTiles + i) * 32 + lane] = make_float4(x[0], x[1], x[2], x[3]);
                 }
-#pragma unroll
-                for (int w = 0; w < F::kGroups; ++w) {
-                    f0[w] = f0[w] == -INFINITY ? 0.0f : ex2(f0[w] - top0);
-                    f1[w] = f1[w] == -INFINITY ? 0.0f : ex2(f1[w] - top1);
-                    sum0 += s_sum[w * kRows + row] * f0[w];
-                    sum1 += s_sum[w * kRows + row + 8] * f1[w];
+                if (rd == 0 && col0 == 0 && (lane & 3) == 0) {
+                    s_max[group * kRows + row] = m0;
+                    s_max[group * kRows + row + 8] = m1;
+                    s_sum[group * kRows + row] = l0;
+                    s_sum[group * kRows + row + 8] = l1;
                 }
-                if (whole) {
-                    const float inv0 = sum0 == 0.0f ? 0.0f : 1.0f / sum0, inv1 = sum1 == 0.0f ? 0.0f : 1.0f / sum1;
+                __syncthreads();
+                if (rd == 0) {
 #pragma unroll
                     for (int w = 0; w < F::kGroups; ++w) {
-                        f0[w] *= inv0;
-                        f1[w] *= inv1;
+                        f0[w] = s_max[w * kRows + row];
+                        f1[w] = s_max[w * kRows + row + 8];
+                        top0 = fmaxf(top0, f0[w]);
+                        top1 = fmaxf(top1, f1[w]);
+                    }
+#pragma unroll
+                    for (int w = 0; w < F::kGroups; ++w) {
+                        f0[w] = f0[w] == -INFINITY ? 0.0f : ex2(f0[w] - top0);
+                        f1[w] = f1[w] == -INFINITY ? 0.0f : ex2(f1[w] - top1);
+                        sum0 += s_sum[w * kRows + row] * f0[w];
+                        sum1 += s_sum[w * kRows + row + 8] * f1[w];
+                    }
+                    if (whole) {
+                        const float inv0 = sum0 == 0.0f ? 0.0f : 1.0f / sum0, inv1 = sum1 == 0.0f ? 0.0f : 1.0f / sum1;
+#pragma unroll
+                        for (int w = 0; w < F::kGroups; ++w) {
+                            f0[w] *= inv0;
+                            f1[w] *= inv1;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    const int mine = rd * kPer + i, nt = tile_of(mine), half = nt / F::kTiles, in_half = nt % F::kTiles - rd * kRoundTiles;
+                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                    for (int w = 0; w < F::kGroups; ++w) {
+                        const int from = ((w * F::kHalves + half) * kRoundTiles + in_half) * 32 + lane;
+                        float4 y;
+                        if (kLow) {
+                            const float2 z = merge2[from];
+                            y = make_float4(z.x, z.y, 0.0f, 0.0f);
+                        } else {
+                            y = merge[from];
+                        }
+                        x.x = fmaf(y.x, f0[w], x.x);
+                        x.y = fmaf(y.y, f0[w], x.y);
+                        x.z = fmaf(y.z, f1[w], x.z);
+                        x.w = fmaf(y.w, f1[w], x.w);
+                    }
+                    if (whole) {
+                        row0.write(a, nt, gates[mine][0], x.x, x.y);
+                        if (!kLow) row1.write(a, nt, gates[mine][1], x.z, x.w);
+                    } else {
+                        __stcg(reinterpret_cast<float4*>(part) + nt * 32 + lane, x);
                     }
                 }
             }
-#pragma unroll
-            for (int i = 0; i < F::kWarpTiles / F::kRounds; ++i) {
-                const int tile = i * F::kWarps + warp, half = tile / F::kRoundTiles, in_half = tile % F::kRoundTiles;
-                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-                for (int w = 0; w < F::kGroups; ++w) {
-                    const float4 y = merge[((w * F::kHalves + half) * F::kRoundTiles + in_half) * 32 + lane];
-                    x.x = fmaf(y.x, f0[w], x.x);
-                    x.y = fmaf(y.y, f0[w], x.y);
-                    x.z = fmaf(y.z, f1[w], x.z);
-                    x.w = fmaf(y.w, f1[w], x.w);
-                }
-                const int mine = rd * (F::kWarpTiles / F::kRounds) + i, nt = tile_of(mine);
-                if (whole) {
-                    write(r_first < rows, out0 + nt * 8, gates[mine][0], x.x, x.y);
-                    write(r_first + 8 < rows, out1 + nt * 8, gates[mine][1], x.z, x.w);
-                } else {
-                    __stcg(reinterpret_cast<float4*>(part) + nt * 32 + lane, x);
-                }
-            }
-        }
-        if (!whole) {
-            if (warp == 0 && (lane & 3) == 0) {
+        };
+        if (low_rows <= 8) add_warps(std::true_type{});
+        else add_warps(std::false_type{});
+        if (!whole && warp == 0) {
+            if ((lane & 3) == 0) {
                 float* ml = part + kRows * D;
                 __stcg(ml + row, top0);
                 __stcg(ml + row + 8, top1);
                 __stcg(ml + kRows + row, sum0);
                 __stcg(ml + kRows + row + 8, sum1);
             }
-            auto part_of = [&](int i) { return p.parts + (size_t)((first + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats; };
-            // whether this block is the last of n at a counter, which is then at zero again
-            auto last_of = [&](unsigned int* counter, int n) {
-                __threadfence();
-                __syncthreads();
-                if (tid == 0) {
-                    s_word[0] = atomicAdd(counter, 1u) == (unsigned)(n - 1);
-                    if (s_word[0]) *counter = 0u;
-                }
-                __syncthreads();
-                const bool last = s_word[0] != 0;
-                if (last) __threadfence();
-                return last;
-            };
-            float* weight = reinterpret_cast<float*>(merge);            // [part][row], then the rows' 1 / sum behind them
-            // adds parts i0, i0 + by, ...: into the result, or into part i0
-            auto add_parts = [&](int i0, int by, int n, bool final) {
-                if (final) ask_gates();
-                if (warp == 0) {
-                    const int r = lane & 15;
-                    float m[kMaxAdded / 2], l[kMaxAdded / 2], top = -INFINITY, sum = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < kMaxAdded / 2; ++j) {
-                        const int i = 2 * j + (lane >> 4);
-                        const float* ml = part_of(i0 + min(i, n - 1) * by) + kRows * D;
-                        m[j] = i < n ? __ldcg(ml + r) : -INFINITY;
-                        l[j] = __ldcg(ml + kRows + r);
-                    }
-#pragma unroll
-                    for (int j = 0; j < kMaxAdded / 2; ++j) top = fmaxf(top, m[j]);
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-#pragma unroll
-                    for (int j = 0; j < kMaxAdded / 2; ++j) {
-                        const int i = 2 * j + (lane >> 4);
-                        const float f = m[j] == -INFINITY ? 0.0f : ex2(m[j] - top);
-                        if (i < n) weight[i * kRows + r] = f;
-                        sum += f * l[j];
-                    }
-                    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-                    if (lane < 16) weight[n * kRows + r] = !final ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
-                    __syncwarp();
-                    if (!final && lane < 16) {
-                        __stcg(part_of(i0) + kRows * D + r, top);
-                        __stcg(part_of(i0) + kRows * D + kRows + r, sum);
-                    }
-                }
-                __syncthreads();
-                constexpr int kT = F::kWarpTiles, kP = 16 / kT;      // loads under way: 16 of 16 bytes a thread
-                const float w0n = weight[n * kRows + row], w1n = weight[n * kRows + row + 8];
-                float4 x[kT];
-#pragma unroll
-                for (int t = 0; t < kT; ++t) x[t] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (int i = 0; i < n; i += kP) {
-                    float4 y[kP][kT];
-#pragma unroll
-                    for (int j = 0; j < kP; ++j) {
-                        const float4* from = reinterpret_cast<const float4*>(part_of(i0 + min(i + j, n - 1) * by)) + lane;
-#pragma unroll
-                        for (int t = 0; t < kT; ++t) y[j][t] = __ldcg(from + tile_of(t) * 32);
-                    }
-#pragma unroll
-                    for (int j = 0; j < kP; ++j) {
-                        if (i + j >= n) continue;
-                        const float w0 = weight[(i + j) * kRows + row], w1 = weight[(i + j) * kRows + row + 8];
-#pragma unroll
-                        for (int t = 0; t < kT; ++t) {
-                            x[t].x = fmaf(y[j][t].x, w0, x[t].x);
-                            x[t].y = fmaf(y[j][t].y, w0, x[t].y);
-                            x[t].z = fmaf(y[j][t].z, w1, x[t].z);
-                            x[t].w = fmaf(y[j][t].w, w1, x[t].w);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < kT; ++t) {
-                    if (final) {
-                        write(r_first < rows, out0 + tile_of(t) * 8, gates[t][0], x[t].x * w0n, x[t].y * w0n);
-                        write(r_first + 8 < rows, out1 + tile_of(t) * 8, gates[t][1], x[t].z * w1n, x[t].w * w1n);
-                    } else {
-                        __stcg(reinterpret_cast<float4*>(part_of(i0)) + tile_of(t) * 32 + lane, x[t]);
-                    }
-                }
-            };
-            const Join join = join_of(count);
-            const int my_run = ((int)blockIdx.x - first) / join.run_len, in_run = min(join.run_len, count - my_run * join.run_len);
-            if (last_of(p.counters + run_counter(first, my_run, join.run_len), in_run)) {
-                if (join.runs == 1) {
-                    add_parts(0, 1, count, true);
-                } else {
-                    if (in_run > 1) add_parts(my_run * join.run_len, 1, in_run, false);
-                    if (last_of(p.counters + item_counter(first), join.runs)) add_parts(0, join.run_len, join.runs, true);
-                }
-            }
         }
         if (F::kHalves == 2) __syncthreads();        // the next item's scores go where the results were added
-        more = at.next_item(p, c0, c1);
+        clear();
     }
     if (!TMA) cp_async_wait<0>();
 }
 
-template <int D, bool TMA>
-cudaError_t launch(const CUtensorMap& tmk, const CUtensorMap& tmv, const DecodeParams& p, int blocks, cudaStream_t s) {
+// Adds the parts of split items in the order of their blocks.  A kernel of its own behind the other one: there the last block to arrive would
+// read up to a hundred parts of 16 KB through one SM (17 us for a single long sequence, in two levels).  Here an item's 8-column tiles are spread over
+// blocks.  Few parts: a warp for each tile, all its parts under way at once.  Many: a block for one or two tiles, its warps share the parts.
+constexpr int kJoinWarps = 8, kJoinAhead = 10;
+template <int D>
+__global__ void __launch_bounds__(kJoinWarps * 32, 2)
+paged_join_kernel(const __grid_constant__ DecodeParams p, int blocks) {
+    constexpr int kTiles = D == 256 ? 2 : 1, kSlices = D / 8 / kTiles, kFewSlices = D / 8 / kJoinWarps;
+    __shared__ SplitItem s_item[kMaxBlocks];
+    __shared__ int s_first[kMaxBlocks], s_count[2][kMaxBlocks / 32];
+    __shared__ unsigned short s_work[kMaxBlocks * kSlices];             // item, slice: item * kSlices + slice
+    __shared__ float4 s_sum[kJoinWarps][kTiles][32];
+    __shared__ float s_top[kJoinWarps][kRows], s_den[kJoinWarps][kRows];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, row = lane >> 2;
+    ptx::griddep_launch_dependents();
+    ptx::griddep_wait();
+    static_assert(kMaxBlocks == kJoinWarps * 32, "a thread looks at a block");
+    static_assert(kMaxBlocks * kSlices <= 65536, "16-bit work numbers");
+    SplitItem mine{};
+    if (tid < blocks) {
+        const int4 x = __ldcg(reinterpret_cast<const int4*>(p.split + tid));
+        mine.count = x.x; mine.q0 = x.y; mine.rows = x.z; mine.head = x.w;
+        mine.tile = __ldcg(&p.split[tid].tile);
+    }
+    // items and pieces of work in front of this thread's
+    const int slices = mine.count == 0 ? 0 : mine.count <= kJoinAhead ? kFewSlices : kSlices;
+    int upto = slices;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+    }
+    const unsigned int vote = __ballot_sync(0xffffffffu, mine.count > 0);
+    if (lane == 31) {
+        s_count[0][warp] = __popc(vote);
+        s_count[1][warp] = upto;
+    }
+    __syncthreads();
+    int works = 0, item0 = __popc(vote & ((1u << lane) - 1u)), work0 = upto - slices;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+        if (w < warp) {
+            item0 += s_count[0][w];
+            work0 += s_count[1][w];
+        }
+        works += s_count[1][w];
+    }
+    if (mine.count > 0) {
+        s_item[item0] = mine;
+        s_first[item0] = tid;
+        for (int i = 0; i < slices; ++i) s_work[work0 + i] = (unsigned short)(item0 * kSlices + i);
+    }
+    __syncthreads();
+    for (int work = blockIdx.x; work < works; work += gridDim.x) {
+        const int number = s_work[work], slice = number % kSlices;
+        const SplitItem it = s_item[number / kSlices];
+        const int first = s_first[number / kSlices];
+        const Row row0(p.a, it.q0, it.rows, it.head, it.tile * kRows + row), row1(p.a, it.q0, it.rows, it.head, it.tile * kRows + row + 8);
+        if (it.count <= kJoinAhead) {
+            const int tile = slice * kJoinWarps + warp;
+            const uint32_t gate0 = row0.gate(p.a, tile), gate1 = row1.gate(p.a, tile);
+            float4 y[kJoinAhead];
+            float m[kJoinAhead / 2], l[kJoinAhead / 2], top = -INFINITY, den = 0.0f;      // part 2j + lane / 16, row lane % 16, in place j
+#pragma unroll
+            for (int j = 0; j < kJoinAhead; ++j)
+                y[j] = __ldcg(reinterpret_cast<const float4*>(p.parts + (size_t)part_slot(first, first + min(j, it.count - 1)) * kPartFloats) + tile * 32 + lane);
+#pragma unroll
+            for (int j = 0; j < kJoinAhead / 2; ++j) {
+                const int i = 2 * j + (lane >> 4);
+                const float* ml = p.parts + (size_t)part_slot(first, first + min(i, it.count - 1)) * kPartFloats + kRows * D + (lane & 15);
+                m[j] = i < it.count ? __ldcg(ml) : -INFINITY;
+                l[j] = i < it.count ? __ldcg(ml + kRows) : 0.0f;
+                top = fmaxf(top, m[j]);
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+#pragma unroll
+            for (int j = 0; j < kJoinAhead / 2; ++j) {
+                m[j] = m[j] == -INFINITY ? 0.0f : ex2(m[j] - top);
+                den += m[j] * l[j];
+            }
+            den += __shfl_xor_sync(0xffffffffu, den, 16);
+            const float norm = den == 0.0f ? 0.0f : 1.0f / den;
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int j = 0; j < kJoinAhead; ++j) {
+                const float w0 = __shfl_sync(0xffffffffu, m[j / 2], j % 2 * 16 + row), w1 = __shfl_sync(0xffffffffu, m[j / 2], j % 2 * 16 + row + 8);
+                if (j >= it.count) continue;
+                x.x = fmaf(y[j].x, w0, x.x);
+                x.y = fmaf(y[j].y, w0, x.y);
+                x.z = fmaf(y[j].z, w1, x.z);
+                x.w = fmaf(y[j].w, w1, x.w);
+            }
+            const float n0 = __shfl_sync(0xffffffffu, norm, row), n1 = __shfl_sync(0xffffffffu, norm, row + 8);
+            row0.write(p.a, tile, gate0, x.x * n0, x.y * n0);
+            row1.write(p.a, tile, gate1, x.z * n1, x.w * n1);
+            continue;
+        }
+        const int tile0 = slice * kTiles;
+        uint32_t gates[2] = {0u, 0u};
+        if (warp < kTiles) {
+            gates[0] = row0.gate(p.a, tile0 + warp);
+            gates[1] = row1.gate(p.a, tile0 + warp);
+        }
+        // parts warp, warp + 8, ...; maxima and sums: part 2j + lane / 16 of these, row lane % 16, in place j
+        float top = -INFINITY, den = 0.0f;           // of row lane % 16 over this half's parts, then over all of the warp's
+        float4 x[kTiles];
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) x[t] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int i0 = warp; i0 < it.count; i0 += kJoinWarps * kJoinAhead) {
+            float4 y[kJoinAhead][kTiles];
+            float m[kJoinAhead / 2], l[kJoinAhead / 2];
+#pragma unroll
+            for (int j = 0; j < kJoinAhead; ++j) {
+                const int i = min(i0 + j * kJoinWarps, it.count - 1);
+                const float4* from = reinterpret_cast<const float4*>(p.parts + (size_t)part_slot(first, first + i) * kPartFloats) + tile0 * 32 + lane;
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) y[j][t] = __ldcg(from + t * 32);
+            }
+#pragma unroll
+            for (int j = 0; j < kJoinAhead / 2; ++j) {
+                const int i = i0 + (2 * j + (lane >> 4)) * kJoinWarps;
+                const float* ml = p.parts + (size_t)part_slot(first, first + min(i, it.count - 1)) * kPartFloats + kRows * D + (lane & 15);
+                m[j] = i < it.count ? __ldcg(ml) : -INFINITY;
+                l[j] = i < it.count ? __ldcg(ml + kRows) : 0.0f;
+            }
+            float now = top;
+#pragma unroll
+            for (int j = 0; j < kJoinAhead / 2; ++j) now = fmaxf(now, m[j]);
+            now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, 16));
+            const float back = top == -INFINITY ? 0.0f : ex2(top - now);
+            top = now;
+            den *= back;
+#pragma unroll
+            for (int j = 0; j < kJoinAhead / 2; ++j) {
+                m[j] = m[j] == -INFINITY ? 0.0f : ex2(m[j] - now);
+                den += m[j] * l[j];
+            }
+            const float b0 = __shfl_sync(0xffffffffu, back, row), b1 = __shfl_sync(0xffffffffu, back, row + 8);
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) x[t] = make_float4(x[t].x * b0, x[t].y * b0, x[t].z * b1, x[t].w * b1);
+#pragma unroll
+            for (int j = 0; j < kJoinAhead; ++j) {
+                const float w0 = __shfl_sync(0xffffffffu, m[j / 2], j % 2 * 16 + row), w1 = __shfl_sync(0xffffffffu, m[j / 2], j % 2 * 16 + row + 8);
+                if (i0 + j * kJoinWarps >= it.count) continue;
+#pragma unroll
+                for (int t = 0; t < kTiles; ++t) {
+                    x[t].x = fmaf(y[j][t].x, w0, x[t].x);
+                    x[t].y = fmaf(y[j][t].y, w0, x[t].y);
+                    x[t].z = fmaf(y[j][t].z, w1, x[t].z);
+                    x[t].w = fmaf(y[j][t].w, w1, x[t].w);
+                }
+            }
+        }
+        den += __shfl_xor_sync(0xffffffffu, den, 16);
+        __syncthreads();                             // the work before is out of the shared arrays
+#pragma unroll
+        for (int t = 0; t < kTiles; ++t) s_sum[warp][t][lane] = x[t];
+        if (lane < kRows) {
+            s_top[warp][lane] = top;
+            s_den[warp][lane] = den;
+        }
+        __syncthreads();
+        if (warp < kTiles) {
+            float t0 = -INFINITY, t1 = -INFINITY, d0 = 0.0f, d1 = 0.0f;
+            float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int w = 0; w < kJoinWarps; ++w) {
+                t0 = fmaxf(t0, s_top[w][row]);
+                t1 = fmaxf(t1, s_top[w][row + 8]);
+            }
+#pragma unroll
+            for (int w = 0; w < kJoinWarps; ++w) {
+                const float a0 = s_top[w][row], a1 = s_top[w][row + 8];
+                const float w0 = a0 == -INFINITY ? 0.0f : ex2(a0 - t0), w1 = a1 == -INFINITY ? 0.0f : ex2(a1 - t1);
+                const float4 v = s_sum[w][warp][lane];
+                d0 += w0 * s_den[w][row];
+                d1 += w1 * s_den[w][row + 8];
+                sum.x = fmaf(v.x, w0, sum.x);
+                sum.y = fmaf(v.y, w0, sum.y);
+                sum.z = fmaf(v.z, w1, sum.z);
+                sum.w = fmaf(v.w, w1, sum.w);
+            }
+            const float n0 = d0 == 0.0f ? 0.0f : 1.0f / d0, n1 = d1 == 0.0f ? 0.0f : 1.0f / d1;
+            row0.write(p.a, tile0 + warp, gates[0], sum.x * n0, sum.y * n0);
+            row1.write(p.a, tile0 + warp, gates[1], sum.z * n1, sum.w * n1);
+        }
+    }
+}
+
+template <class... P, class... A>
+cudaError_t launch_behind(void (*kernel)(P...), int grid, int threads, int smem, cudaStream_t s, const A&... args) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(Form<D>::kThreads);
-    cfg.dynamicSmemBytes = Form<D>::kSmem;
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_decode_kernel<D, TMA>, tmk, tmv, p);
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <int D>
-cudaError_t launch(const DecodeParams& p, int blocks, cudaStream_t s) {
+cudaError_t launch(const DecodeParams& p, const nvfp4_device_info& dev, cudaStream_t s) {
+    const int blocks = dev.sm_count < kMaxBlocks ? dev.sm_count : kMaxBlocks, parts = p.piece == kGroup ? Form<D>::kWidth / 64 : 1;
     CUtensorMap tmk{}, tmv{};
-    if (p.piece && make_cache_map(&tmk, p.a.b, p.a.b.k, p.piece, p.piece == kGroup ? Form<D>::kWidth / 64 : 1) &&
-        make_cache_map(&tmv, p.a.b, p.a.b.v, p.piece, p.piece == kGroup ? Form<D>::kWidth / 64 : 1))
-        return launch<D, true>(tmk, tmv, p, blocks, s);
-    return launch<D, false>(tmk, tmv, p, blocks, s);
+    cudaError_t e;
+    if (p.piece && make_cache_map(&tmk, p.a.b, p.a.b.k, p.piece, parts) && make_cache_map(&tmv, p.a.b, p.a.b.v, p.piece, parts))
+        e = launch_behind(paged_decode_kernel<D, true>, blocks, Form<D>::kThreads, Form<D>::kSmem, s, tmk, tmv, p);
+    else
+        e = launch_behind(paged_decode_kernel<D, false>, blocks, Form<D>::kThreads, Form<D>::kSmem, s, tmk, tmv, p);
+    if (e != cudaSuccess) return e;
+    return launch_behind(paged_join_kernel<D>, 2 * blocks, kJoinWarps * 32, 0, s, p, blocks);
 }
 
 }  // namespace
@@ -693,7 +830,7 @@ bool make_cache_map(CUtensorMap* m, const paged::Batch& b, const void* base, int
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-size_t paged_scratch_bytes(int sm_count) { return kCounterBytes + (size_t)sm_count * 2 * kPartFloats * sizeof(float); }
+size_t paged_scratch_bytes(int sm_count) { return kSplitBytes + (size_t)(sm_count < kMaxBlocks ? sm_count : kMaxBlocks) * 2 * kPartFloats * sizeof(float); }
 
 cudaError_t configure_paged_decode() {
     cudaError_t e = configure_large_smem(paged_decode_kernel<64, true>, Form<64>::kSmem);
@@ -709,14 +846,13 @@ cudaError_t launch_paged_decode(const paged::AttentionArgs& a, const nvfp4_devic
     DecodeParams p{};
     p.a = a;
     p.scale_log2 = a.scale * 1.4426950408889634f;
-    p.min_cost = 4;
+    p.min_cost = 3;
     p.most_rows = 0x7fffffff;
     p.piece = a.b.page_size % 16 == 0 ? 16 : a.b.page_size % 8 == 0 ? 8 : 0;
-    p.counters = static_cast<unsigned int*>(scratch);
-    p.parts = reinterpret_cast<float*>(static_cast<char*>(scratch) + kCounterBytes);
-    const int blocks = dev.sm_count < kMaxBlocks ? dev.sm_count : kMaxBlocks;
-    *launches = 1;
-    return a.b.head_dim == 64 ? launch<64>(p, blocks, s) : a.b.head_dim == 128 ? launch<128>(p, blocks, s) : launch<256>(p, blocks, s);
+    p.split = static_cast<SplitItem*>(scratch);
+    p.parts = reinterpret_cast<float*>(static_cast<char*>(scratch) + kSplitBytes);
+    *launches = 2;
+    return a.b.head_dim == 64 ? launch<64>(p, dev, s) : a.b.head_dim == 128 ? launch<128>(p, dev, s) : launch<256>(p, dev, s);
 }
 
 }  // namespace nvfp4

@@ -111,7 +111,7 @@ constexpr int kRows = 16;
 // What an item costs beside its units (its rows of q, the warps' sums, the result's way out) is about kItemCost units, so that a run of
 // many short items would take several times as long as a run of a long one: runs are cut in places of cost, of which an item has
 // kItemCost in front of its units.  A window of more than kItemCost places holds a unit, so no run is without one.
-constexpr int kItemCost = 1;
+constexpr int kItemCost = 2;
 struct Items {
     int tiles, items, chunks;
     NVFP4_PAGED_HD int cost() const { return chunks + kItemCost; }              // of one item
@@ -139,26 +139,10 @@ NVFP4_PAGED_HD Units units_in(long long at, const Items& n, long long c0, long l
     const long long u = at + kItemCost;
     return {(int)least(most(c0 - u, 0LL), (long long)n.chunks), (int)least(most(c1 - u, 0LL), (long long)n.chunks)};
 }
-// The blocks that hold parts of a split item, first .. first + count - 1, count in at counters.  Up to kFlatParts parts are added by the block
-// that arrives last; more in two levels: runs of about the square root of their count by the last block of each run, then the runs' sums by the last of
-// those.  An item's first block is no other split item's first one, but its last block may be the next item's first: counters of the first
-// runs and of the second level go by `first`, those of later runs by the run's first block in a range of their own.
-constexpr int kMaxBlocks = 256, kFlatParts = 10, kMaxAdded = 16;      // kMaxAdded^2 >= kMaxBlocks: parts that one block adds at most
-constexpr int kCounters = 3 * kMaxBlocks;
-struct Join {
-    int run_len, runs;
-};
-NVFP4_PAGED_HD Join join_of(int count) {
-    Join j{count, 1};
-    if (count > kFlatParts) {
-        j.run_len = 1;
-        while (j.run_len * j.run_len < count) ++j.run_len;
-        j.runs = (count + j.run_len - 1) / j.run_len;
-    }
-    return j;
-}
-NVFP4_PAGED_HD int run_counter(int first, int run, int run_len) { return run == 0 ? first : 2 * kMaxBlocks + first + run * run_len; }
-NVFP4_PAGED_HD int item_counter(int first) { return kMaxBlocks + first; }
+// An item that several blocks share is held in parts by blocks first .. first + count - 1: the first one's part, the only one of an item that
+// begins in that block and is split, in its slot 1, the others' in their slots 0.
+constexpr int kMaxBlocks = 256;
+NVFP4_PAGED_HD int part_slot(int first, int block) { return 2 * block + (block == first ? 1 : 0); }
 
 // ---- checks of the calls' arguments
 inline bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }

@@ -58,8 +58,8 @@ int paged_sequence(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int s, i
 }
 
 // Walks the runs of all blocks over the batch's places of cost.  0: runs are in order and together all places, each holds a unit; the units of every
-// item are shared among the blocks from that of its first unit to that of its last one, each of which has at least one, each unit once; no two counts
-// of a launch share a counter and no block adds more parts than there is room for.
+// item are shared among the blocks from that of its first unit to that of its last one, each of which has at least one, each unit once; no two
+// parts of split items share a slot.
 int paged_walk(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int group, int chunk, int grid, int min_cost) {
     Batch x{};
     if (check_batch(c, b, &x)) return 1;
@@ -78,7 +78,7 @@ int paged_walk(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int group, i
     const int blocks = blocks_of(cost, grid, min_cost);
     if (blocks < 1 || blocks > grid) return 2;
     if (run_begin(cost, blocks, 0) != 0 || run_begin(cost, blocks, blocks) != cost) return 3;
-    std::vector<int> used(kCounters, 0), held(blocks, 0), slots(2 * blocks, 0);
+    std::vector<int> held(blocks, 0), slots(2 * blocks, 0);
     for (size_t i = 0; i < at.size(); ++i) {
         const Items& n = items[i];
         const int first = block_of(cost, blocks, at[i] + kItemCost), last = block_of(cost, blocks, at[i] + kItemCost + n.chunks - 1);
@@ -91,19 +91,12 @@ int paged_walk(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int group, i
             if (u.from != next) return 6;
             next = u.to;
             ++held[k];
-            if (last > first && ++slots[2 * k + (k == first)] > 1) return 7;
+            if (last > first && ++slots[part_slot(first, k)] > 1) return 7;
         }
         if (next != n.chunks) return 8;
-        if (last == first) continue;
-        const Join j = join_of(last - first + 1);
-        if (j.run_len < 1 || j.runs < 1 || (long long)j.run_len * j.runs < last - first + 1 || j.run_len * (j.runs - 1) >= last - first + 1) return 9;
-        if (j.run_len > kMaxAdded || j.runs > kMaxAdded) return 10;
-        for (int r = 0; r < j.runs; ++r)
-            if (++used[run_counter(first, r, j.run_len)] > 1) return 11;
-        if (j.runs > 1 && ++used[item_counter(first)] > 1) return 12;
     }
     for (int k = 0; k < blocks; ++k)
-        if (!held[k]) return 13;
+        if (!held[k]) return 9;
     return 0;
 }
 
