@@ -296,7 +296,7 @@ int nvfp4_create(int device, size_t workspace_bytes, nvfp4_handle** out) {
     workspace_bytes &= ~(size_t)255;     // everything carved out of the workspace, from either end, stays 256-byte aligned
     e = cudaMalloc(&h->workspace, workspace_bytes);
     if (e == cudaSuccess) e = cudaMemset(h->workspace, 0, workspace_bytes);
-    const size_t paged_bytes = paged_scratch_bytes(h->dev.sm_count);
+    const size_t paged_bytes = paged_scratch_bytes(h->dev.sm_count) + paged_prefill_scratch_bytes(h->dev.sm_count);
     if (e == cudaSuccess) e = cudaMalloc(&h->paged_scratch, paged_bytes);
     if (e == cudaSuccess) e = cudaMemset(h->paged_scratch, 0, paged_bytes);
     if (e == cudaSuccess) e = configure_kernels(h->dev);
@@ -785,8 +785,21 @@ int nvfp4_paged_attention(nvfp4_handle* h, const nvfp4_paged_attention_desc* d, 
     a.b.status = reinterpret_cast<unsigned int*>(h->workspace);
     OnDevice on(h->dev.device);
     if (on.e != cudaSuccess) return (int)on.e;
+    // Up to 16 rows (new tokens x heads of a group) of a sequence share one tile of the few-token kernel, which runs at the rate of the
+    // cache's bytes; a tcgen05 tile holds 128.  The host knows bounds only: where they leave no room for sequences of both kinds, one kernel
+    // takes all, otherwise each takes its own.
+    constexpr int kFewRows = paged::kRows;
+    cudaError_t e = cudaSuccess;
     int nl = 0;
-    const cudaError_t e = launch_paged_decode(a, h->dev, h->paged_scratch, &nl, stream);
+    bool all = true;                 // the few-token kernel takes every sequence
+    if ((long long)a.b.max_q_len * a.group > kFewRows && paged_prefill_supported(a)) {
+        const bool one_kind = a.b.sequences == 1 || (long long)a.b.sequences * a.b.max_q_len == a.b.tokens;
+        char* scratch = h->paged_scratch + paged_scratch_bytes(h->dev.sm_count);
+        all = !launch_paged_prefill(a, one_kind ? 0 : kFewRows, h->dev, scratch, &nl, stream, &e);
+        h->launches += (unsigned long long)nl;
+        if (!all && (one_kind || e != cudaSuccess)) return cuda_status(e);
+    }
+    e = launch_paged_decode(a, all ? 0x7fffffff : kFewRows, h->dev, h->paged_scratch, &nl, stream);
     h->launches += (unsigned long long)nl;
     return cuda_status(e);
 }

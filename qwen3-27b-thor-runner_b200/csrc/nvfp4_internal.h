@@ -210,10 +210,16 @@ cudaError_t launch_skinny_umma(const LinearArgs& a, nvfp4_device_info& dev, void
 
 // --- the paged cache (paged_plan.h has the calls' arguments): kv_append.cu, paged_decode.cu.
 cudaError_t launch_kv_append(const paged::AppendArgs& a, const nvfp4_device_info& dev, int* launches, cudaStream_t s);
-// The attention's own scratch: joins of split sequences.  Zeroed once; every launch leaves its counters at zero.
+// The attention's own scratch: the parts of split items.
 size_t paged_scratch_bytes(int sm_count);
 cudaError_t configure_paged_decode();
-cudaError_t launch_paged_decode(const paged::AttentionArgs& a, const nvfp4_device_info& dev, void* scratch, int* launches, cudaStream_t s);
+// Sequences with up to most_rows (new tokens x group) rows.
+cudaError_t launch_paged_decode(const paged::AttentionArgs& a, int most_rows, const nvfp4_device_info& dev, void* scratch, int* launches, cudaStream_t s);
+// paged_prefill.cu: sequences with more than above_rows rows, on tcgen05.  False: the call cannot be described to the TMA unit, nothing is launched.
+size_t paged_prefill_scratch_bytes(int sm_count);
+cudaError_t configure_paged_prefill();
+bool paged_prefill_supported(const paged::AttentionArgs& a);
+bool launch_paged_prefill(const paged::AttentionArgs& a, int above_rows, const nvfp4_device_info& dev, void* scratch, int* launches, cudaStream_t s, cudaError_t* e);
 
 cudaError_t configure_kernels(nvfp4_device_info& dev);
 

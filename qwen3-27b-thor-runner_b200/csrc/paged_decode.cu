@@ -842,12 +842,12 @@ cudaError_t configure_paged_decode() {
     return e;
 }
 
-cudaError_t launch_paged_decode(const paged::AttentionArgs& a, const nvfp4_device_info& dev, void* scratch, int* launches, cudaStream_t s) {
+cudaError_t launch_paged_decode(const paged::AttentionArgs& a, int most_rows, const nvfp4_device_info& dev, void* scratch, int* launches, cudaStream_t s) {
     DecodeParams p{};
     p.a = a;
     p.scale_log2 = a.scale * 1.4426950408889634f;
     p.min_cost = 3;
-    p.most_rows = 0x7fffffff;
+    p.most_rows = most_rows;
     p.piece = a.b.page_size % 16 == 0 ? 16 : a.b.page_size % 8 == 0 ? 8 : 0;
     p.split = static_cast<SplitItem*>(scratch);
     p.parts = reinterpret_cast<float*>(static_cast<char*>(scratch) + kSplitBytes);

@@ -144,6 +144,57 @@ NVFP4_PAGED_HD Units units_in(long long at, const Items& n, long long c0, long l
 constexpr int kMaxBlocks = 256;
 NVFP4_PAGED_HD int part_slot(int first, int block) { return 2 * block + (block == first ? 1 : 0); }
 
+// ---- work of the attention of many tokens.  An item is a (sequence, tile of tile_tokens new tokens, key-value head); its units are the
+// kLongChunk keys wide chunks that its last token sees, so a prompt's tiles have more and more of them.  Items in order (sequence, tile, head) have
+// kLongCost places of cost in front of their units and are cut into runs as above.
+constexpr int kLongChunk = 128, kLongCost = 2;
+
+// sum of floor((a i + b) / m) over 0 <= i < n (a, b >= 0, m > 0), by swapping slope and modulus as in Euclid's algorithm
+NVFP4_PAGED_HD long long floor_sum(long long n, unsigned m, unsigned a, unsigned b) {
+    long long sum = 0;
+    while (n > 0) {
+        sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
+        a %= m;
+        b %= m;
+        const unsigned long long top = (unsigned long long)a * n + b;
+        if (top < m) break;
+        n = (long long)(top / m);
+        b = (unsigned)(top % m);
+        const unsigned t = m;
+        m = a;
+        a = t;
+    }
+    return sum;
+}
+
+struct LongItems {
+    int tiles, tile_tokens, heads;
+};
+NVFP4_PAGED_HD LongItems long_items_of(const Batch& b, const Sequence& q, int group, int tile_tokens, int above_rows) {
+    LongItems n{0, tile_tokens, b.kv_heads};
+    if ((long long)q.q_len * group > above_rows) n.tiles = (q.q_len + tile_tokens - 1) / tile_tokens;
+    return n;
+}
+// Keys that the last token of a tile sees, and the tile's units (one at least: rows that see nothing have a result too).
+NVFP4_PAGED_HD int long_limit(const Sequence& q, const LongItems& n, int tile) {
+    return sees(q, (int)least((long long)(tile + 1) * n.tile_tokens, (long long)q.q_len) - 1);
+}
+NVFP4_PAGED_HD int long_chunks(int limit) { return most((limit + kLongChunk - 1) / kLongChunk, 1); }
+// Places of the first `tiles` tiles of one head.
+NVFP4_PAGED_HD long long long_places(const Sequence& q, const LongItems& n, int tiles) {
+    const long long full = least(tiles, n.tiles - 1), step = n.tile_tokens;       // tiles whose last token is (i + 1) * step - 1
+    long long sum = (long long)tiles * kLongCost;
+    if (tiles == n.tiles && tiles > 0) sum += long_chunks(long_limit(q, n, tiles - 1));
+    if (full <= 0) return sum;
+    // first + (i + 1) * step keys: up to kLongChunk of them one chunk, beyond kv those that kv has
+    const long long ones = kLongChunk - q.first < 0 ? 0 : least(((long long)kLongChunk - q.first) / step, full);
+    const long long open = (long long)q.kv - q.first < 0 ? 0 : least(((long long)q.kv - q.first) / step, full);
+    sum += ones;
+    if (open > ones) sum += floor_sum(open - ones, kLongChunk, (unsigned)step, (unsigned)(q.first + (ones + 1) * step + kLongChunk - 1));
+    const long long past = full - most(open, ones);
+    return sum + past * long_chunks(q.kv);
+}
+
 // ---- checks of the calls' arguments
 inline bool aligned(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 

@@ -985,6 +985,7 @@ cudaError_t configure_kernels(nvfp4_device_info& dev) {
     if (e == cudaSuccess) e = configure_decode_fp4();
     if (e == cudaSuccess) e = configure_decode_fp4_stream();
     if (e == cudaSuccess) e = configure_paged_decode();
+    if (e == cudaSuccess) e = configure_paged_prefill();
     return e;
 }
 

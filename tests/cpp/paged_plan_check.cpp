@@ -57,6 +57,29 @@ int paged_sequence(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int s, i
     return 0;
 }
 
+// Places of a sequence's first tiles in closed form against the sum over them: the number of tiles at which the two differ.
+int paged_long_places(int q_len, int kv_len, int max_kv, int tile_tokens) {
+    Batch x{};
+    x.tokens = q_len;
+    x.kv_heads = 1;
+    x.sequences = 1;
+    x.max_kv = max_kv;
+    const int cu[2] = {0, q_len};
+    x.cu_q = cu;
+    x.kv_len = &kv_len;
+    const Sequence q = sequence(x, 0);
+    const LongItems n = long_items_of(x, q, 1, tile_tokens, 0);
+    long long sum = 0;
+    int bad = long_places(q, n, 0) != 0;
+    for (int t = 0; t < n.tiles; ++t) {
+        const int limit = long_limit(q, n, t);
+        if (limit < 0 || limit > q.kv) return -1;
+        sum += long_chunks(limit) + kLongCost;
+        bad += long_places(q, n, t + 1) != sum;
+    }
+    return bad;
+}
+
 // Walks the runs of all blocks over the batch's places of cost.  0: runs are in order and together all places, each holds a unit; the units of every
 // item are shared among the blocks from that of its first unit to that of its last one, each of which has at least one, each unit once; no two
 // parts of split items share a slot.

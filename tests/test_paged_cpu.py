@@ -210,3 +210,14 @@ def test_every_unit_has_one_block(lib):
         c, b = arrays(kv, np.zeros((n, 400), np.int32), cu=np.cumsum([0] + new), tokens=sum(new) + 1, page_size=16, kv_heads=rng.choice([1, 2, 8]))
         got = lib.paged_walk(ctypes.byref(c), ctypes.byref(b), rng.choice([1, 3, 12, 16]), rng.choice([64, 128]), rng.choice([1, 2, 148, 256]), rng.choice([3, 4, 9]))
         assert got == 0, (got, new, kv)
+
+
+def test_places_of_causal_tiles(lib):
+    """The closed form of the units of a prompt's tiles: behind a past, at its own start, with rows in front of position 0, cut off by the page table."""
+    rng = random.Random(12)
+    for _ in range(3000):
+        q = rng.choice([1, 2, 127, 128, 129, rng.randint(1, 300), rng.randint(1, 9000)])
+        kv = rng.choice([0, q, q + rng.randint(0, 300), q + rng.randint(0, 200000), rng.randint(0, q), -5, 2147483647])
+        max_kv = rng.choice([2147418111, rng.randint(1, 400), rng.randint(1, 20000)])
+        step = rng.choice([1, 2, 10, 21, 32, 128, 256, rng.randint(1, 256)])
+        assert lib.paged_long_places(q, kv, max_kv, step) == 0, (q, kv, max_kv, step)
