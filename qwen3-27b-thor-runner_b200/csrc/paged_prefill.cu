@@ -32,6 +32,9 @@ namespace nvfp4 {
 
 bool make_cache_map(CUtensorMap* m, const paged::Batch& b, const void* base, int slots, int parts);
 
+#ifndef NVFP4_NT
+#define NVFP4_NT 2
+#endif
 namespace {
 
 using namespace paged;
@@ -42,18 +45,21 @@ template <int D>
 struct Form {
     static constexpr int kSlotBytes = D == 64 ? 16384 : 32768;
     static constexpr int kWidth = D == 64 ? 64 : 128;            // elements of a slot of keys
-    static constexpr int kNT = D == 256 ? 1 : 2;                 // tiles of an item
-    static constexpr int kThreads = 96 + 128 * kNT;
+    static constexpr int kNT = D == 256 ? 1 : NVFP4_NT;                 // tiles of an item
+    static constexpr int kThreads = 96 + 256;
+    static constexpr int kBufs = kNT == 2 ? 1 : D == 256 ? 2 : 3;       // buffers of scores of a tile
     static constexpr int kParts = D / kWidth;                    // slots of a unit's keys, and of its values
     static constexpr int kQTile = kTile * D * 2;
     static constexpr int kSlots = (224 * 1024 - kNT * kQTile) / kSlotBytes;
     static constexpr int kVTokens = kLongChunk / kParts;         // tokens of a slot of values
-    static constexpr int kOCol = 256, kOStep = D == 64 ? 64 : 128;
-    static constexpr int kSmem = kNT * kQTile + kSlots * kSlotBytes + 1024 + 1024;
+    static constexpr int kSCols = kNT == 2 ? 256 : kBufs * 128;  // columns of scores, those of results behind them
+    static constexpr int kOCol = kSCols, kOStep = D == 64 ? 64 : 128;
+    static constexpr int kOkRing = kSlots / kParts > 8 ? 16 : 8; // units whose page masks are kept: more than the ring holds
+    static constexpr int kControl = 2048;
+    static constexpr int kSmem = kNT * kQTile + kSlots * kSlotBytes + kControl + 1024;
 };
 static_assert(Form<256>::kSmem <= 232448 && Form<64>::kSmem <= 232448, "shared memory");
 constexpr int kMaxPartFloats = kTile * 260;          // results, maxima and sums of one tile of 256 columns or two of 128
-constexpr int kOkRing = 16;          // units whose page masks are kept: more than the ring holds
 
 struct LongSplit {
     int count, q0, q_len, tile, head;
@@ -259,17 +265,18 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
     uint64_t* empty = full + F::kSlots;
     uint64_t* q_full = empty + F::kSlots;
     uint64_t* q_empty = q_full + 1;
-    uint64_t* s_full = q_empty + 1;                  // [2] scores are there
-    uint64_t* p_ready = s_full + 2;                  // [2] weights are there, results scaled to them
-    uint64_t* s_free = p_ready + 2;                  // [2] the weights are multiplied
-    uint64_t* o_free = s_free + 2;                   // [2] the item's results are read, tile by tile
+    uint64_t* s_full = q_empty + 1;                  // [3] scores are there
+    uint64_t* p_ready = s_full + 3;                  // [3] weights are there, results scaled to them
+    uint64_t* s_free = p_ready + 3;                  // [3] the weights are multiplied
+    uint64_t* o_free = s_free + 3;                   // [2] the item's results are read, tile by tile
     uint64_t* drain = o_free + 2;                    // [2] the issuers' last MMAs
     uint32_t* s_tmem = reinterpret_cast<uint32_t*>(drain + 2);
     volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem + 1);
     unsigned int* s_ok = s_tmem + 2;                 // [kOkRing] boxes of a unit whose page is one
-    long long* prefix = reinterpret_cast<long long*>(s_ok + kOkRing);                   // [warps] in front, then the run's first place
+    long long* prefix = reinterpret_cast<long long*>(s_ok + F::kOkRing);                   // [warps] in front, then the run's first place
     Cursor<D>* found = reinterpret_cast<Cursor<D>*>(prefix + F::kThreads / 32 + 2);
-    static_assert((2 * F::kSlots + 12) * 8 + 8 + kOkRing * 4 + (F::kThreads / 32 + 2) * 8 + sizeof(Cursor<D>) <= 1024, "control block");
+    float* s_x = reinterpret_cast<float*>(found + 1);                                   // [group][row], one tile: what the two groups tell each other
+    static_assert((2 * F::kSlots + 15) * 8 + 8 + F::kOkRing * 4 + (F::kThreads / 32 + 2) * 8 + sizeof(Cursor<D>) + 2 * kTile * 4 <= F::kControl, "control block");
 
     const AttentionArgs& a = p.a;
     const Batch& b = a.b;
@@ -278,7 +285,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
         for (int i = 0; i < F::kSlots; ++i) { ptx::mbar_init(&full[i], 1); ptx::mbar_init(&empty[i], 1); }
         ptx::mbar_init(q_full, 1);
         ptx::mbar_init(q_empty, 1);
-        for (int i = 0; i < 2; ++i) { ptx::mbar_init(&s_full[i], 1); ptx::mbar_init(&p_ready[i], 4); ptx::mbar_init(&s_free[i], 1); ptx::mbar_init(&o_free[i], 4); ptx::mbar_init(&drain[i], 1); }
+        for (int i = 0; i < 3; ++i) { ptx::mbar_init(&s_full[i], 1); ptx::mbar_init(&p_ready[i], 8 / F::kNT); ptx::mbar_init(&s_free[i], 1); }
+        for (int i = 0; i < 2; ++i) { ptx::mbar_init(&o_free[i], 8 / F::kNT); ptx::mbar_init(&drain[i], 1); }
         *s_abort = 0;
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&tmq);
@@ -392,7 +400,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
         // lane = (64 elements, box of tokens)
         auto keys = [&](int page, int place) {
             const unsigned int ok = __ballot_sync(0xffffffffu, page >= 0);
-            if (lane == 0) s_ok[unit % kOkRing] = ok;
+            if (lane == 0) s_ok[unit % F::kOkRing] = ok;
             ++unit;
             const int box = lane % boxes, part = lane / boxes;
             const int pg = __shfl_sync(0xffffffffu, page, box), pl = __shfl_sync(0xffffffffu, place, box);
@@ -477,17 +485,16 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
                 for (int t = 0; t < F::kNT; ++t) {
                     if (t >= live) continue;
                     const uint32_t u = units_of[t] + j;
-                    const int sb = F::kNT == 1 ? u & 1u : t;
+                    const int sb = F::kNT == 1 ? u % F::kBufs : t;
                     const bool release = t == live - 1;
                     // the unit's keys (values) come in this half of the ring's fills
                     const unsigned int half = used + (F::kNT == 2 ? 2 * j + !is_s : is_s ? (j ? 2 * j - 1 : 0) : (j < n - 1 ? 2 * j + 2 : 2 * n - 1));
                     if (is_s) {
                         // the buffer's weights before are multiplied
-                        if (F::kNT == 1 && u >= 2) wait(&s_free[sb], (u >> 1) - 1 & 1u, 0xA38u);
-                        if (F::kNT == 2 && u >= 1) wait(&s_free[sb], u - 1 & 1u, 0xA38u);
+                        if (u >= F::kBufs) wait(&s_free[sb], u / F::kBufs - 1 & 1u, 0xA38u);
                     } else {
                         if (j == 0 && items_of[t] > 0) wait(&o_free[t], items_of[t] - 1 & 1u, 0xA34u);
-                        wait(&p_ready[sb], F::kNT == 1 ? u >> 1 & 1u : u & 1u, 0xA35u);
+                        wait(&p_ready[sb], u / F::kBufs & 1u, 0xA35u);
                     }
                     for (int c = 0; c < F::kParts; ++c) {
                         const unsigned int i = half * F::kParts + c;
@@ -526,11 +533,23 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
         ptx::mbar_wait(&drain[!is_s], 0, s_abort, b.status, 0xA3Fu);
     } else {
         // ------------------------------------------------------------------ softmax: thread = row
-        const int t = (warp - 3) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+        // Two tiles: a group of four warps each, thread = row.  One tile: the two groups share it, thread = row and 64 of the scores, half the result.
+        constexpr bool kShared = F::kNT == 1;
+        constexpr int kCols = kShared ? 64 : 128;
+        const int g = (warp - 3) >> 2, t = kShared ? 0 : g, quarter = warp & 3, row = quarter * 32 + lane, s_col = kShared ? g * 64 : 0;
+        const int col0 = kShared ? g * (D / 2) : 0, col1 = kShared ? col0 + D / 2 : D;
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16), o_addr = lanes + F::kOCol + t * F::kOStep;
         uint32_t unit = 0;                           // of this tile so far
         unsigned int used = 0;
         uint32_t units_seen = 0;                     // of the block, for the page masks
+        // the other group's value of this row
+        auto exchange = [&](float x) {
+            s_x[g * kTile + row] = x;
+            ptx::named_barrier_sync(1 + quarter, 64);
+            const float y = s_x[(1 - g) * kTile + row];
+            ptx::named_barrier_sync(1 + quarter, 64);
+            return y;
+        };
         while (more) {
             const int n = at.to - at.chunk;
             const bool live = t < at.live(p);
@@ -543,15 +562,15 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
                 p.split[blockIdx.x] = LongSplit{block_of(cost, blocks, at.at + kLongCost + at.chunks - 1) - first + 1, at.q.q0, at.q.q_len, at.tile, at.head, {0, 0, 0}};
             float m = -INFINITY, l = 0.0f;
             for (int j = 0; live && j < n; ++j, ++unit) {
-                const int sb = F::kNT == 1 ? unit & 1 : t;
-                const uint32_t par = F::kNT == 1 ? unit >> 1 & 1u : unit & 1u, s_addr = lanes + sb * 128;
-                ptx::mbar_wait(&s_full[sb], par, s_abort, b.status, 0xA40u);
+                const int sb = F::kNT == 1 ? unit % F::kBufs : t;
+                const uint32_t s_addr = lanes + sb * 128;
+                ptx::mbar_wait(&s_full[sb], unit / F::kBufs & 1u, s_abort, b.status, 0xA40u);
                 __syncwarp();
                 umma::tc_fence_after();
                 const int key0 = (at.chunk + j) * kLongChunk;
-                const unsigned int ok = s_ok[(units_seen + j) % kOkRing], all = (1u << (kLongChunk / p.k_rows)) - 1u;
+                const unsigned int ok = s_ok[(units_seen + j) % F::kOkRing], all = (1u << (kLongChunk / p.k_rows)) - 1u;
                 if (key0 + kLongChunk > at.limit || ok != all) {
-                    if (t == 0) {
+                    if (t == 0 && (!kShared || D > 64 || g == 0)) {
                         // values of keys that no row sees: whatever lies there, a weight of zero times it is to be zero
                         const int box = row / p.k_rows;
                         const bool none = key0 + row >= at.limit || !(ok >> box & 1u);
@@ -562,7 +581,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
                         if (none) {
                             const uint32_t to = ptx::smem_u32(ring + slot * F::kSlotBytes) + row % F::kVTokens * 128;
 #pragma unroll
-                            for (int c = 0; c < D / 64; ++c)
+                            for (int c = kShared && D > 64 ? g * (D / 128) : 0; c < (kShared && D > 64 ? (g + 1) * (D / 128) : D / 64); ++c)
 #pragma unroll
                                 for (int e = 0; e < 8; ++e)
                                     asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(to + c * (F::kVTokens * 128) + e * 16), "r"(0u) : "memory");
@@ -571,43 +590,44 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
                         __syncwarp();
                     }
                 }
-                uint32_t s[128];
+                uint32_t s[kCols];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) tmem_ld32(s_addr + q * 32, s + q * 32);
+                for (int q = 0; q < kCols / 32; ++q) tmem_ld32(s_addr + s_col + q * 32, s + q * 32);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) tmem_wait_ld32(s + q * 32);
-                const int seen = see - key0;         // columns in front of this one
-                const bool masked = __any_sync(0xffffffffu, there && seen < kLongChunk) || ok != all;
+                for (int q = 0; q < kCols / 32; ++q) tmem_wait_ld32(s + q * 32);
+                const int seen = see - key0 - s_col; // of this thread's columns those in front of this one
+                const bool masked = __any_sync(0xffffffffu, there && seen < kCols) || ok != all;
                 auto mask = [&](int q) {
                     const int box_log = 31 - __clz(p.k_rows);
                     unsigned int keep = seen >= q * 32 + 32 ? 0xffffffffu : seen <= q * 32 ? 0u : (1u << (seen - q * 32)) - 1u;
-                    if (!(ok >> ((q * 32) >> box_log) & 1u)) keep &= 0xffff0000u;
-                    if (!(ok >> ((q * 32 + 16) >> box_log) & 1u)) keep &= 0x0000ffffu;
+                    if (!(ok >> ((s_col + q * 32) >> box_log) & 1u)) keep &= 0xffff0000u;
+                    if (!(ok >> ((s_col + q * 32 + 16) >> box_log) & 1u)) keep &= 0x0000ffffu;
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         if (!(keep >> i & 1u)) s[q * 32 + i] = 0xff800000u;
                 };
                 if (masked) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) mask(q);
+                    for (int q = 0; q < kCols / 32; ++q) mask(q);
                 }
                 float top[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top[i] = fmaxf(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
 #pragma unroll
-                for (int i = 8; i < 128; i += 2) top[i / 2 & 3] = max3(top[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-                const float now = max3(fmaxf(top[0], top[1]), top[2], top[3]) * p.scale_log2;
+                for (int i = 8; i < kCols; i += 2) top[i / 2 & 3] = max3(top[i / 2 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+                float now = max3(fmaxf(top[0], top[1]), top[2], top[3]) * p.scale_log2;
+                if (kShared) now = fmaxf(now, exchange(now));
                 if (__any_sync(0xffffffffu, there && now > m + 8.0f)) {
                     const float next = fmaxf(m, now), back = next == m ? 1.0f : ex2(m - next);
                     m = next;
                     l *= back;
                     if (j > 0) {                     // the results so far follow, once the product before is through
                         const uint32_t u = unit - 1;
-                        ptx::mbar_wait(&s_free[F::kNT == 1 ? u & 1u : t], F::kNT == 1 ? u >> 1 & 1u : u & 1u, s_abort, b.status, 0xA42u);
+                        ptx::mbar_wait(&s_free[F::kNT == 1 ? u % F::kBufs : t], u / F::kBufs & 1u, s_abort, b.status, 0xA42u);
                         __syncwarp();
                         umma::tc_fence_after();
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
+                        for (int c = col0; c < col1; c += 32) {
                             uint32_t x[32];
                             tmem_ld32(o_addr + c, x);
                             tmem_wait_ld32(x);
@@ -621,11 +641,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
                 const uint64_t scale2 = pair(p.scale_log2, p.scale_log2), base2 = pair(-base, -base);
                 uint64_t sum[2] = {0, 0};            // two sums each
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
+                for (int q = 0; q < kCols / 32; ++q) {
                     uint32_t w[16];
                     if (q == 3) {
-                        tmem_wait_ld32(s + 96);
-                        if (masked) mask(3);
+                        tmem_wait_ld32(s + q * 32);
+                        if (masked) mask(q);
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
@@ -636,9 +656,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
                         sum[i & 1] = add2(sum[i & 1], pair(x, y));
                         w[i] = pack_bf16(x, y);
                     }
-                    tmem_st16(s_addr + q * 16, w);   // over scores that are read
-                    // two tiles' threads have 168 registers: the last 32 scores are read again rather than kept
-                    if (q == 0) tmem_ld32(s_addr + 96, s + 96);
+                    tmem_st16(s_addr + s_col / 2 + q * 16, w);         // over scores that are read
+                    // 128 scores and the weights pass the 168 registers of 352 threads: the last 32 are read again rather than kept
+                    if (kCols == 128 && q == 0) tmem_ld32(s_addr + 96, s + 96);
                 }
                 {
                     float x, y;
@@ -657,24 +677,28 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
                 const uint32_t u = unit - 1;
                 const long long tq = at.q.q0 + tok, out_at = tq * a.o_stride + (long long)hd * a.o_head, gate_at = tq * a.g_stride + (long long)hd * a.g_head;
                 uint4 gates[2][4];                   // asked for 32 columns ahead
-                ask_gates(a, there && whole, gate_at, gates[0]);
-                ptx::mbar_wait(&s_free[F::kNT == 1 ? u & 1u : t], F::kNT == 1 ? u >> 1 & 1u : u & 1u, s_abort, b.status, 0xA43u);
+                ask_gates(a, there && whole, gate_at + col0, gates[0]);
+                ptx::mbar_wait(&s_free[F::kNT == 1 ? u % F::kBufs : t], u / F::kBufs & 1u, s_abort, b.status, 0xA43u);
                 __syncwarp();
                 umma::tc_fence_after();
+                if (kShared) {
+                    const float other = exchange(l);
+                    l = g == 0 ? l + other : other + l;
+                }
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
                 float* part = p.parts + (size_t)part_slot(first, blockIdx.x) * kMaxPartFloats;
                 const int prow = t * kTile + row;
 #pragma unroll 2
-                for (int c = 0; c < D; c += 32) {
+                for (int c = col0; c < col1; c += 32) {
                     uint32_t x[32];
                     tmem_ld32(o_addr + c, x);
-                    if (c + 32 < D) ask_gates(a, there && whole, gate_at + c + 32, gates[(c / 32 + 1) & 1]);
+                    if (c + 32 < col1) ask_gates(a, there && whole, gate_at + c + 32, gates[((c - col0) / 32 + 1) & 1]);
                     tmem_wait_ld32(x);
                     if (whole) {
                         float y[32];
 #pragma unroll
                         for (int i = 0; i < 32; ++i) y[i] = l == 0.0f ? 0.0f : __uint_as_float(x[i]) * inv;
-                        if (there) write32(a, out_at + c, gates[c / 32 & 1], y);
+                        if (there) write32(a, out_at + c, gates[(c - col0) / 32 & 1], y);
                         __syncwarp();
                     } else {
 #pragma unroll
@@ -683,7 +707,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
                                    make_float4(__uint_as_float(x[4 * i]), __uint_as_float(x[4 * i + 1]), __uint_as_float(x[4 * i + 2]), __uint_as_float(x[4 * i + 3])));
                     }
                 }
-                if (!whole) {
+                if (!whole && col0 == 0) {
                     float* ml = part + F::kNT * kTile * D;
                     __stcg(ml + prow, m);
                     __stcg(ml + F::kNT * kTile + prow, l);
