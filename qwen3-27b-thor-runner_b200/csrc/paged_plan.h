@@ -149,18 +149,19 @@ NVFP4_PAGED_HD int part_slot(int first, int block) { return 2 * block + (block =
 // kLongCost places of cost in front of their units and are cut into runs as above.
 constexpr int kLongChunk = 128, kLongCost = 2;
 
-// sum of floor((a i + b) / m) over 0 <= i < n (a, b >= 0, m > 0), by swapping slope and modulus as in Euclid's algorithm
-NVFP4_PAGED_HD long long floor_sum(long long n, unsigned m, unsigned a, unsigned b) {
+// sum of floor((a i + b) / m) over 0 <= i < n (m > 0, a (n - 1) + b and a mod m * n + b mod m below 2^32), by swapping slope and modulus as in
+// Euclid's algorithm
+NVFP4_PAGED_HD long long floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
     long long sum = 0;
     while (n > 0) {
-        sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
+        sum += (long long)n * (n - 1) / 2 * (a / m) + (long long)n * (b / m);
         a %= m;
         b %= m;
-        const unsigned long long top = (unsigned long long)a * n + b;
+        const uint32_t top = a * n + b;
         if (top < m) break;
-        n = (long long)(top / m);
-        b = (unsigned)(top % m);
-        const unsigned t = m;
+        n = top / m;
+        b = top % m;
+        const uint32_t t = m;
         m = a;
         a = t;
     }
@@ -182,17 +183,17 @@ NVFP4_PAGED_HD int long_limit(const Sequence& q, const LongItems& n, int tile) {
 NVFP4_PAGED_HD int long_chunks(int limit) { return most((limit + kLongChunk - 1) / kLongChunk, 1); }
 // Places of the first `tiles` tiles of one head.
 NVFP4_PAGED_HD long long long_places(const Sequence& q, const LongItems& n, int tiles) {
-    const long long full = least(tiles, n.tiles - 1), step = n.tile_tokens;       // tiles whose last token is (i + 1) * step - 1
+    const int full = least(tiles, n.tiles - 1), step = n.tile_tokens;             // tiles whose last token is (i + 1) * step - 1
     long long sum = (long long)tiles * kLongCost;
     if (tiles == n.tiles && tiles > 0) sum += long_chunks(long_limit(q, n, tiles - 1));
     if (full <= 0) return sum;
     // first + (i + 1) * step keys: up to kLongChunk of them one chunk, beyond kv those that kv has
-    const long long ones = kLongChunk - q.first < 0 ? 0 : least(((long long)kLongChunk - q.first) / step, full);
-    const long long open = (long long)q.kv - q.first < 0 ? 0 : least(((long long)q.kv - q.first) / step, full);
+    const int ones = least((int)least(most((long long)kLongChunk - q.first, 0LL), 0x7fffffffLL) / step, full);
+    const int open = least((int)least(most((long long)q.kv - q.first, 0LL), 0x7fffffffLL) / step, full);
     sum += ones;
-    if (open > ones) sum += floor_sum(open - ones, kLongChunk, (unsigned)step, (unsigned)(q.first + (ones + 1) * step + kLongChunk - 1));
-    const long long past = full - most(open, ones);
-    return sum + past * long_chunks(q.kv);
+    if (open > ones) sum += floor_sum((uint32_t)(open - ones), kLongChunk, (uint32_t)step, (uint32_t)(q.first + (ones + 1) * step + kLongChunk - 1));
+    const int past = full - most(open, ones);
+    return sum + (long long)past * long_chunks(q.kv);
 }
 
 // ---- checks of the calls' arguments
