@@ -147,7 +147,7 @@ NVFP4_PAGED_HD int part_slot(int first, int block) { return 2 * block + (block =
 // ---- work of the attention of many tokens.  An item is a (sequence, tile of tile_tokens new tokens, key-value head); its units are the
 // kLongChunk keys wide chunks that its last token sees, so a prompt's tiles have more and more of them.  Items in order (sequence, tile, head) have
 // kLongCost places of cost in front of their units and are cut into runs as above.
-constexpr int kLongChunk = 128, kLongCost = 2;
+constexpr int kLongChunk = 128, kLongCost = 6;
 
 // sum of floor((a i + b) / m) over 0 <= i < n (m > 0, a (n - 1) + b and a mod m * n + b mod m below 2^32), by swapping slope and modulus as in
 // Euclid's algorithm

@@ -71,7 +71,7 @@ struct PrefillParams {
     float scale_log2;
     int above_rows;                  // sequences with no more rows belong to another kernel
     int tile_tokens;                 // new tokens of a tile: 128 / group
-    int box_rows;                    // tokens of a box of keys or values
+    int box_rows, box_log;           // tokens of a box of keys or values (16, 32 or 64)
     int min_cost;
     LongSplit* split;
     float* parts;
@@ -230,22 +230,46 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return d;
 }
 
-// 32 columns of a row's result, gated, rounded once.
-__device__ __forceinline__ void write32(const AttentionArgs& a, long long out_at, const uint4* g, const uint32_t (&x)[32]) {
+__device__ __forceinline__ float min_nan(float x, float y) {             // NaN stays NaN
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(x), "f"(y));
+    return d;
+}
+// Two values times the sigmoids of their BF16 gates, 1 / (1 + u) with u = 2^(-log2(e) gate).  2^x and 1 / x come from the same unit, four values a clock and
+// scheduler, which would be all that a tile's way out waits for: one reciprocal, of (1 + u) (1 + v), serves both.  u stays below 2^63 for that: a gate
+// below -43.6 counts as -43.6, a factor of 1e-19.
+__device__ __forceinline__ uint32_t gated(float x, float y, uint32_t gate) {
+    const float c = -1.4426950408889634f;
+    const float u = 1.0f + min_nan(ex2(__uint_as_float(gate << 16) * c), 0x1p63f), v = 1.0f + min_nan(ex2(__uint_as_float(gate & 0xFFFF0000u) * c), 0x1p63f);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(u * v));
+    return pack_bf16(x * (v * r), y * (u * r));
+}
+// 16 rows and 32 columns: register 4 i + 2 h + e of a lane is row lane / 4 + 8 h, column 8 i + 2 (lane % 4) + e.
+__device__ __forceinline__ void tmem_ld16x32(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : NVFP4_R8(r, 0), NVFP4_R8(r, 8)
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {        // of all loads so far, r's among them
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 ::"memory");
+}
+// Among four lanes: word k of lane c becomes word c of lane k.
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
+    const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float y[8];
+    for (int i = 0; i < 4; i += 2) {
+        const uint32_t x = __shfl_xor_sync(0xffffffffu, odd ? w[i] : w[i + 1], 1);
+        if (odd) w[i] = x; else w[i + 1] = x;
+    }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = __uint_as_float(x[i * 8 + e]);
-        if (a.gate) {
-            const uint32_t w[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                y[2 * e] = __fdividef(y[2 * e], 1.0f + __expf(-__uint_as_float(w[e] << 16)));
-                y[2 * e + 1] = __fdividef(y[2 * e + 1], 1.0f + __expf(-__uint_as_float(w[e] & 0xFFFF0000u)));
-            }
-        }
-        *reinterpret_cast<uint4*>(a.out + out_at + i * 8) = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t x = __shfl_xor_sync(0xffffffffu, high ? w[i] : w[i + 2], 2);
+        if (high) w[i] = x; else w[i + 2] = x;
     }
 }
 
@@ -381,7 +405,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
     if (warp == 0) {
         // ------------------------------------------------------------------ producer
         int slot = 0;
-        unsigned int unit = 0, tails = 0;
+        unsigned int unit = 0, tails = 0, tail_ok = 0;
+        int tail_slot = -1, tail_left = 0;
         uint32_t phase = 0, q_phase = 0;
         const int boxes = kLongChunk / p.box_rows, mine = boxes / 2;                     // of a unit; of its keys in this CTA
         const uint32_t full0 = ptx::mapa_shared(ptx::smem_u32(full), 0), q_full0 = ptx::mapa_shared(ptx::smem_u32(q_full), 0);
@@ -445,19 +470,28 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
                 if (lane == 0) ptx::mbar_arrive_expect_tx(tail, (unsigned)(__popc(ok) * p.box_rows * F::kVCols * 2));
                 __syncwarp();
                 if (go) ptx::tma_load_5d(to + part * (kLongChunk * 128) + box * p.box_rows * 128, &tmv, tail, 0, pl, cols, at.head, pg);
-                const bool there = ptx::mbar_wait(tail, tails & 1u, s_abort, b.status, 0xA24u);
-                ++tails;
-                if (!there) return;
-                for (int tok = lane; tok < kLongChunk; tok += 32)
-                    if (tok >= left || !(ok >> (tok / p.box_rows) & 1u)) {
-                        for (int i = 0; i < kAcross * 8; ++i)
-                            *reinterpret_cast<uint4*>(to + (i >> 3) * (kLongChunk * 128) + tok * 128 + (i & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                    }
-                ptx::fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive_cluster_release(full0 + slot * 8);
+                tail_slot = slot;
+                tail_left = left;
+                tail_ok = ok;
             }
             next_slot();
+        };
+        // The values that a tail load brought are zeroed in part and then count; the next item's queries may be asked for in between.
+        auto finish_tail = [&]() {
+            if (tail_slot < 0) return;
+            const bool there = ptx::mbar_wait(tail, tails & 1u, s_abort, b.status, 0xA24u);
+            ++tails;
+            unsigned char* to = ring + tail_slot * F::kSlotBytes;
+            constexpr int kPer = F::kVCols / 8;                                          // 16-byte pieces of a token
+            for (int i = lane; there && i < kLongChunk * kPer; i += 32) {
+                const int tok = i / kPer, piece = i % kPer;
+                if (tok >= tail_left || !(tail_ok >> (tok >> p.box_log) & 1u))
+                    *reinterpret_cast<uint4*>(to + (piece >> 3) * (kLongChunk * 128) + tok * 128 + (piece & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive_cluster_release(full0 + tail_slot * 8);
+            tail_slot = -1;
         };
         while (more) {
             int page, place, page_before = -1, place_before = 0;
@@ -473,12 +507,14 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
                                               at.q.q0 + at.tile * at.n.tile_tokens + (2 * t + rank) * p.tile_tokens);
             }
             __syncwarp();
+            finish_tail();
             for (int j = at.chunk; j < at.to; ++j) {
                 int page_next = -1, place_next = 0;
                 if (j + 1 < at.to) look_up(j + 1, page_next, place_next);
                 keys(page, place);
                 if (F::kNT == 2) values(j, page, place);
                 else if (j > at.chunk) values(j - 1, page_before, place_before);
+                if (F::kNT == 1 || j + 1 < at.to) finish_tail();         // pages out of bounds in the middle; the last unit's waits for the next queries
                 page_before = page;
                 place_before = place;
                 page = page_next;
@@ -487,6 +523,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
             if (F::kNT == 1) values(at.to - 1, page_before, place_before);
             more = at.next_item(p, c0, c1);
         }
+        finish_tail();
         // nothing of this CTA's may still be on its way when it ends: every slot's last fill has been multiplied
         for (int i = 0; i < F::kSlots; ++i) {
             ptx::mbar_wait(&empty[slot], phase ^ 1u, s_abort, b.status, 0xA23u);
@@ -564,6 +601,14 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
         const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
         const uint32_t p_ready0 = ptx::mapa_shared(ptx::smem_u32(p_ready), 0), o_free0 = ptx::mapa_shared(ptx::smem_u32(o_free), 0);
         const unsigned int all = (1u << (kLongChunk / p.box_rows)) - 1u;
+        const int in_tile = row / a.group;           // token of the tile
+        // rows lane / 4 + 8 r of the warp's 32: token of the tile and head of the group
+        int out_tok[4], out_head[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            out_tok[r] = (quarter * 32 + r * 8 + (lane >> 2)) / a.group;
+            out_head[r] = quarter * 32 + r * 8 + (lane >> 2) - out_tok[r] * a.group;
+        }
         uint32_t units_of[2] = {0, 0};               // of a tile so far
         uint32_t units_seen = 0;                     // for the page masks
         int turn = 0;
@@ -576,19 +621,19 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
             return to[(1 - g) * kTile];
         };
         while (more) {
-            const int n = at.to - at.chunk, live = at.live(p), in_tile = row / a.group, hd = at.head * a.group + row - in_tile * a.group;
+            const int n = at.to - at.chunk, live = at.live(p);
             const bool whole = at.chunk == 0 && at.to == at.chunks;
-            const int first = block_of(cost, pairs, at.at + kLongCost);
+            const int first = whole ? id : block_of(cost, pairs, at.at + kLongCost);
             if (!whole && first == id && rank == 0 && tid == 96)
                 p.split[id] = LongSplit{block_of(cost, pairs, at.at + kLongCost + at.chunks - 1) - first + 1, at.q.q0, at.q.q_len, at.tile, at.head, {0, 0, 0}};
-            int tok[F::kNT], see[F::kNT];
+            int see[F::kNT];
             bool there[F::kNT];
             float m[F::kNT], l[F::kNT];
 #pragma unroll
             for (int t = 0; t < F::kNT; ++t) {
-                tok[t] = at.tile * at.n.tile_tokens + (2 * t + rank) * p.tile_tokens + in_tile;
-                there[t] = in_tile < p.tile_tokens && tok[t] < at.q.q_len;
-                see[t] = there[t] ? sees(at.q, tok[t]) : 0x7fffffff;
+                const int tok = at.tile * at.n.tile_tokens + (2 * t + rank) * p.tile_tokens + in_tile;
+                there[t] = in_tile < p.tile_tokens && tok < at.q.q_len;
+                see[t] = there[t] ? sees(at.q, tok) : 0x7fffffff;
                 m[t] = -INFINITY;
                 l[t] = 0.0f;
             }
@@ -611,12 +656,11 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
                     tmem_wait_ld32(s + 32);
                     const int seen = see[t] - key0 - s_col;      // of this thread's columns those in front of this one
                     if (__any_sync(0xffffffffu, there[t] && seen < 64) || ok != all) {
-                        const int box_log = 31 - __clz(p.box_rows);
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {
                             unsigned int keep = seen >= q * 32 + 32 ? 0xffffffffu : seen <= q * 32 ? 0u : (1u << (seen - q * 32)) - 1u;
-                            if (!(ok >> ((s_col + q * 32) >> box_log) & 1u)) keep &= 0xffff0000u;
-                            if (!(ok >> ((s_col + q * 32 + 16) >> box_log) & 1u)) keep &= 0x0000ffffu;
+                            if (!(ok >> ((s_col + q * 32) >> p.box_log) & 1u)) keep &= 0xffff0000u;
+                            if (!(ok >> ((s_col + q * 32 + 16) >> p.box_log) & 1u)) keep &= 0x0000ffffu;
 #pragma unroll
                             for (int i = 0; i < 32; ++i)
                                 if (!(keep >> i & 1u)) s[q * 32 + i] = 0xff800000u;
@@ -680,29 +724,66 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
                 if (t >= live) continue;
                 units_of[t] += n;
                 const uint32_t u = units_of[t] - 1, o_addr = lanes + F::kOCol + t * 128 + col0;
-                const long long tq = at.q.q0 + tok[t], out_at = tq * a.o_stride + (long long)hd * a.o_head + col0, gate_at = tq * a.g_stride + (long long)hd * a.g_head + col0;
-                uint4 gates[kCols / 8];              // asked for while the last product runs
-                if (a.gate && whole && there[t]) {
+                // A thread's row is 32 lines away from its neighbours': for the way out four lanes take a row instead (row lane / 4 and further ones 8,
+                // 16, 24 on), 16 bytes each, with the row's factor from the thread whose row it is.
+                const int span = at.tile * at.n.tile_tokens + (2 * t + rank) * p.tile_tokens;          // the tile's first token
+                auto goes = [&](int r) { return whole && out_tok[r] < p.tile_tokens && span + out_tok[r] < at.q.q_len; };
+                auto place_of = [&](int r, long long stride, long long head_stride) {
+                    return (long long)(at.q.q0 + span + out_tok[r]) * stride + (long long)(at.head * a.group + out_head[r]) * head_stride + col0 + (lane & 3) * 8;
+                };
+                uint4 gates[kCols / 32][2];          // of two of the four rows, asked for while the last product runs
+                auto ask_gates = [&](int h) {
 #pragma unroll
-                    for (int i = 0; i < kCols / 8; ++i) gates[i] = *reinterpret_cast<const uint4*>(a.gate + gate_at + i * 8);
-                }
+                    for (int r = 0; r < 2; ++r) {
+                        const bool go = a.gate && goes(2 * h + r);
+                        const uint16_t* from = a.gate + (go ? place_of(2 * h + r, a.g_stride, a.g_head) : 0);
+#pragma unroll
+                        for (int c = 0; c < kCols / 32; ++c) gates[c][r] = go ? *reinterpret_cast<const uint4*>(from + c * 32) : make_uint4(0u, 0u, 0u, 0u);
+                    }
+                };
+                ask_gates(0);
                 const float mine_l = l[t], other_l = exchange(mine_l), sum = g == 0 ? mine_l + other_l : other_l + mine_l;
                 ptx::mbar_wait(&s_free[F::kNT == 1 ? u % F::kBufs : t], u / F::kBufs & 1u, s_abort, b.status, 0xA43u);
                 __syncwarp();
                 umma::tc_fence_after();
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 float* part = p.parts + (size_t)(part_slot(first, id) * 2 + rank) * kMaxPartFloats;
+                if (whole) {
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-                for (int c = 0; c < kCols; c += 32) {
-                    uint32_t x[32];
-                    tmem_ld32(o_addr + c, x);
-                    tmem_wait_ld32(x);
-                    if (whole) {
+                    for (int h = 0; h < 2; ++h) {
+                        const float inv_r[2] = {__shfl_sync(0xffffffffu, inv, h * 16 + (lane >> 2)), __shfl_sync(0xffffffffu, inv, h * 16 + 8 + (lane >> 2))};
+                        uint32_t x[kCols / 32][16];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] = sum == 0.0f ? 0u : __float_as_uint(__uint_as_float(x[i]) * inv);
-                        if (there[t]) write32(a, out_at + c, gates + c / 8, x);
-                        __syncwarp();
-                    } else {
+                        for (int c = 0; c < kCols / 32; ++c) tmem_ld16x32(o_addr + ((uint32_t)(h * 16) << 16) + c * 32, x[c]);
+#pragma unroll
+                        for (int c = 0; c < kCols / 32; ++c) tmem_wait_ld16(x[c]);
+#pragma unroll
+                        for (int r = 0; r < 2; ++r) {
+                            const bool go = goes(2 * h + r);
+                            uint16_t* out = a.out + (go ? place_of(2 * h + r, a.o_stride, a.o_head) : 0);
+#pragma unroll
+                            for (int c = 0; c < kCols / 32; ++c) {
+                                uint32_t gate[4] = {gates[c][r].x, gates[c][r].y, gates[c][r].z, gates[c][r].w}, w[4];
+                                if (a.gate) transpose4(gate);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    // rows without a key: zero, whatever the product holds
+                                    const float y = inv_r[r] == 0.0f ? 0.0f : __uint_as_float(x[c][4 * i + 2 * r]) * inv_r[r];
+                                    const float z = inv_r[r] == 0.0f ? 0.0f : __uint_as_float(x[c][4 * i + 2 * r + 1]) * inv_r[r];
+                                    w[i] = a.gate ? gated(y, z, gate[i]) : pack_bf16(y, z);
+                                }
+                                transpose4(w);
+                                if (go) *reinterpret_cast<uint4*>(out + c * 32) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        }
+                        if (h == 0) ask_gates(1);
+                    }
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kCols; c += 32) {
+                        uint32_t x[32];
+                        tmem_ld32(o_addr + c, x);
+                        tmem_wait_ld32(x);
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
                             __stcg(reinterpret_cast<float4*>(part) + (t * (D / 4) + (col0 + c) / 4 + i) * kTile + row,
@@ -816,12 +897,8 @@ paged_prefill_join_kernel(const __grid_constant__ PrefillParams p, int pairs) {
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            float u = x[2 * e] * inv, v = x[2 * e + 1] * inv;
-            if (a.gate) {
-                u = __fdividef(u, 1.0f + __expf(-__uint_as_float(g[e] << 16)));
-                v = __fdividef(v, 1.0f + __expf(-__uint_as_float(g[e] & 0xFFFF0000u)));
-            }
-            w[e] = pack_bf16(u, v);
+            const float u = x[2 * e] * inv, v = x[2 * e + 1] * inv;
+            w[e] = a.gate ? gated(u, v, g[e]) : pack_bf16(u, v);
         }
         *reinterpret_cast<uint4*>(a.out + tq * a.o_stride + hd * a.o_head + c0) = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -870,6 +947,7 @@ bool launch(PrefillParams& p, const nvfp4_device_info& dev, cudaStream_t s, cuda
     CUtensorMap maps[3];
     p.tile_tokens = kTile / p.a.group;
     p.box_rows = common_divisor(p.a.b.page_size, Form<D>::kKeys);
+    p.box_log = p.box_rows == 64 ? 6 : p.box_rows == 32 ? 5 : 4;
     if (!make_q_map(&maps[0], p.a, p.tile_tokens) || !make_cache_map(&maps[1], p.a.b, p.a.b.k, p.box_rows, 1) || !make_cache_map(&maps[2], p.a.b, p.a.b.v, p.box_rows, 1))
         return false;
     const int pairs = pairs_of(dev);
@@ -899,7 +977,7 @@ bool launch_paged_prefill(const paged::AttentionArgs& a, int above_rows, const n
     p.a = a;
     p.scale_log2 = a.scale * 1.4426950408889634f;
     p.above_rows = above_rows;
-    p.min_cost = 4;
+    p.min_cost = kLongCost + 1;
     p.split = static_cast<LongSplit*>(scratch);
     p.parts = reinterpret_cast<float*>(static_cast<char*>(scratch) + kSplitBytes);
     const bool done = a.b.head_dim == 64 ? launch<64>(p, dev, s, e) : a.b.head_dim == 128 ? launch<128>(p, dev, s, e) : launch<256>(p, dev, s, e);
