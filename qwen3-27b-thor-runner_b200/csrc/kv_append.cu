@@ -1,10 +1,11 @@
 // New tokens into the paged cache: norms of queries and keys for each head, rotation by the position, and the writes of keys and
 // values to their places, in one pass (the reference's fused qk-norm-rope and KV-write kernels, src/engine/light_ops.cu).
 //
-// Every value is read once and written once; the arithmetic (an FMA per value for the norm, a product with cos and sin for the
-// rotated part) is nothing beside it.  A head is spread over head_dim / 8 lanes of a warp, 16 bytes a lane, so a norm is a reduction
-// over those lanes and the partner i + rot_dim / 2 of element i lies rot_dim / 16 lanes away, a shuffle.  The angles are the same
-// for all heads of a token: the block's threads compute them once, in shared memory, while the loads are under way.
+// Every value is read once and written once, and the bound should be that; but a value comes with a dozen instructions, so the instructions
+// are what had to go: with a thread for eight neighbours, partners exchanged by shuffles and addresses formed for every head of every token 6534 tokens of 28
+// heads of 256 took 61-79 us.  Now a head is spread over head_dim / 8 lanes; a lane of the part that turns holds four elements and their partners
+// i + rot_dim / 2, and goes through several tokens with the same head.  A norm is a reduction over the head's lanes.  The angles are the same
+// for all heads of a token and computed once, in shared memory, while the loads are under way.
 // position * inv_freq is formed and reduced to [-pi, pi] in FP64 (a float of 2^17 has steps of 1/64: the angle itself would be lost),
 // the reduced angle is rounded to FP32 (1.2e-7) for sincosf.
 #include <cuda_bf16.h>
@@ -40,100 +41,153 @@ __device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// One block per token and run of `per` heads: head x of the token's q_heads + 2 kv_heads (queries, keys, values).
-template <int D, int UNROLL>
+// The sequence of row t, by a whole warp: the last s with cu_q[s] <= t, the range cut into 32 pieces at a time.
+__device__ __forceinline__ bool find_row(const Batch& b, int t, int& seq, int& pos) {
+    if (!b.cu_q) {
+        seq = t;
+        return t < b.sequences && row_position(b, t, t, t + 1, t, pos);
+    }
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = b.sequences;                     // lo <= s < hi
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, s = lo + lane * step;
+        const unsigned int below = __ballot_sync(0xffffffffu, s < hi && b.cu_q[s] <= t);
+        const int k = below ? 31 - __clz(below) : 0;
+        hi = min(lo + (k + 1) * step, hi);
+        lo = lo + k * step;
+    }
+    seq = lo;
+    return row_position(b, lo, b.cu_q[lo], b.cu_q[lo + 1], t, pos);
+}
+
+// One block per TOKENS tokens and run of `per` heads: head x of a token's q_heads + 2 kv_heads (queries, keys, values).  A head's lanes keep it for
+// UNROLL tokens at a time.  The first values are asked for at once; which sequence, length and page a token belongs to, a chain of three loads, and its
+// angles are a warp's work for each token beside them.
+template <int D, int TOKENS, int UNROLL>
 __global__ void __launch_bounds__(kThreads)
 kv_append_kernel(AppendArgs a, int per) {
     constexpr int kLanes = D / 8, kHeads = kThreads / kLanes;      // lanes per head, heads per step of the block
-    __shared__ float2 s_turn[D / 2];
-    const int tid = threadIdx.x, t = blockIdx.x, lane = tid % kLanes;
+    static_assert(TOKENS <= kThreads / 32, "a warp looks a token up");
+    __shared__ float4 s_turn[TOKENS][D / 4];          // cos and sin of two pairs each
+    __shared__ long long s_at[TOKENS];                // place in the cache; -1: none; -2: the row is left out
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid % kLanes, t0 = blockIdx.x * TOKENS;
     const Batch& b = a.b;
     ptx::griddep_launch_dependents();
     ptx::griddep_wait();                              // rows, lengths and table may come from the kernel in front
-    int seq, pos;
-    if (!find_row(b, t, seq, pos)) return;            // the same in the whole block
-    const int total = a.q_heads + 2 * b.kv_heads, end = min(total, (int)(blockIdx.y + 1) * per);
+    const int h0 = blockIdx.y * per, end = min(a.q_heads + 2 * b.kv_heads, h0 + per), tokens = min(TOKENS, b.tokens - t0);
+    // this lane's elements: four and their partners where the head turns, eight in a row behind that
     const int half = a.rot_dim / 2;
-    if (tid < half) {
-        const int p = a.positions ? a.positions[t] : pos;
-        double angle = (double)p * (double)a.inv_freq[tid];
-        angle = fma(-rint(angle * (1.0 / kTwoPi)), kTwoPi, angle);
-        float sn, cs;
-        sincosf((float)angle, &sn, &cs);
-        s_turn[tid] = make_float2(cs, sn);
-    }
-    long long at = -1;
-    if (pos < b.max_kv) at = place(b, seq, pos);
-    if (at < 0 && tid == 0 && blockIdx.y == 0) atomicCAS(b.status, 0u, kStatusPlace);
-    __syncthreads();
-    const int reach = half / 8;                       // lanes between an element and its partner
-    for (int base = blockIdx.y * per + tid / kLanes; base - tid / kLanes < end; base += kHeads * UNROLL) {
-        uint4 x[UNROLL];
+    const bool turns = lane * 8 < a.rot_dim;
+    const int e0 = turns ? lane * 4 : lane * 8, e1 = turns ? half + lane * 4 : lane * 8 + 4;
+    int h = h0 + tid / kLanes;
+    const uint16_t* from = nullptr;
+    long long stride = 0;
+    auto begin_head = [&]() {
+        if (h < a.q_heads) { from = a.q + (long long)h * a.q_head; stride = a.q_stride; }
+        else if (h < a.q_heads + b.kv_heads) { from = a.k + (long long)(h - a.q_heads) * a.k_head; stride = a.k_stride; }
+        else { from = a.v + (long long)(h - a.q_heads - b.kv_heads) * a.v_head; stride = a.v_stride; }
+        from += (long long)t0 * stride;
+    };
+    uint2 x[UNROLL][2];
+    auto ask = [&](int tk) {
 #pragma unroll
         for (int u = 0; u < UNROLL; ++u) {
-            const int head = base + u * kHeads;
-            const uint16_t* from = nullptr;
-            if (head < end) {
-                if (head < a.q_heads) from = a.q + (long long)t * a.q_stride + (long long)head * a.q_head;
-                else if (head < a.q_heads + b.kv_heads) from = a.k + (long long)t * a.k_stride + (long long)(head - a.q_heads) * a.k_head;
-                else from = a.v + (long long)t * a.v_stride + (long long)(head - a.q_heads - b.kv_heads) * a.v_head;
-            }
-            x[u] = from ? *reinterpret_cast<const uint4*>(from + lane * 8) : make_uint4(0u, 0u, 0u, 0u);
+            const bool go = h < end && tk + u < tokens;
+            const uint16_t* at = from + (tk + u) * stride;
+            x[u][0] = go ? *reinterpret_cast<const uint2*>(at + e0) : make_uint2(0u, 0u);
+            x[u][1] = go ? *reinterpret_cast<const uint2*>(at + e1) : make_uint2(0u, 0u);
         }
+    };
+    begin_head();
+    ask(0);
+    if (warp < tokens) {
+        int seq, pos = 0;
+        const bool there = find_row(b, t0 + warp, seq, pos);
+        const int p = a.positions ? a.positions[t0 + warp] : pos;
+        long long at = there ? -1 : -2;
+        if (there && pos < b.max_kv) at = place(b, seq, pos);
+        if ((tid & 31) == 0) {
+            s_at[warp] = at;
+            if (at == -1) atomicCAS(b.status, 0u, kStatusPlace);
+        }
+        for (int i = tid & 31; i < half; i += 32) {
+            double angle = (double)p * (double)a.inv_freq[i];
+            angle = fma(-rint(angle * (1.0 / kTwoPi)), kTwoPi, angle);
+            float sn, cs;
+            sincosf((float)angle, &sn, &cs);
+            reinterpret_cast<float2*>(s_turn[warp])[i] = make_float2(cs, sn);
+        }
+    }
+    __syncthreads();
+    for (int base = h0; base < end; base += kHeads) {
+        if (base != h0) {
+            h = base + tid / kLanes;
+            begin_head();
+            ask(0);
+        }
+        const bool is_q = h < a.q_heads, is_v = h >= a.q_heads + b.kv_heads;
+        const uint16_t* weight = is_v ? nullptr : is_q ? a.q_norm : a.k_norm;
+        float w[8];                                   // 1 + weight
+        if (weight && h < end) {
+            const uint2 w0 = *reinterpret_cast<const uint2*>(weight + e0), w1 = *reinterpret_cast<const uint2*>(weight + e1);
+            unpack8(make_uint4(w0.x, w0.y, w1.x, w1.y), w);
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int head = base + u * kHeads;
-            const bool is_q = head < a.q_heads, is_v = head >= a.q_heads + b.kv_heads;
-            const uint16_t* weight = is_q ? a.q_norm : a.k_norm;
-            uint4 out = x[u];
-            if (__any_sync(0xffffffffu, !is_v)) {
-                float v[8];
-                unpack8(x[u], v);
-                float ss = 0.0f;
+            for (int i = 0; i < 8; ++i) w[i] += 1.0f;
+        }
+        // the head's place in a token's row of q_out or of the cache
+        uint16_t* const to = is_q ? a.q_out + (long long)h * a.o_head : is_v ? b.v + (long long)(h - a.q_heads - b.kv_heads) * b.head_stride : b.k + (long long)(h - a.q_heads) * b.head_stride;
+        for (int tk = 0; tk < tokens; tk += UNROLL) {
+            if (tk) ask(tk);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+            for (int u = 0; u < UNROLL; ++u) {
+                uint4 out = make_uint4(x[u][0].x, x[u][0].y, x[u][1].x, x[u][1].y);
+                const bool go = h < end && tk + u < tokens;
+                if (!is_v) {
+                    float v[8];
+                    unpack8(out, v);
+                    if (weight) {
+                        float ss = 0.0f;
 #pragma unroll
-                for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                if (weight) {
-                    const float inv = 1.0f / sqrtf(ss / (float)D + a.eps);
-                    float w[8];
-                    unpack8(*reinterpret_cast<const uint4*>(weight + lane * 8), w);
+                        for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+                        // the lanes of a head take the branches together
+                        const unsigned int group = kLanes == 32 ? 0xffffffffu : ((1u << (kLanes & 31)) - 1u) << ((tid & 31) / kLanes * kLanes);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * (1.0f + w[i]);
-                }
-                // lanes 0 .. reach-1 hold the first halves of the pairs, the next `reach` lanes the second ones
-                const bool first = lane < reach, turns = lane < 2 * reach;
-                const int partner = (tid & 31) + (first ? reach : turns ? -reach : 0);
-                const float2* turn = s_turn + (first ? lane : turns ? lane - reach : 0) * 8;
+                        for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(group, ss, o);
+                        const float inv = rsqrtf(ss * (1.0f / D) + a.eps);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float other = __shfl_sync(0xffffffffu, v[i], partner);
-                    if (turns) {
-                        const float2 cs = turn[i];
-                        v[i] = first ? v[i] * cs.x - other * cs.y : v[i] * cs.x + other * cs.y;
+                        for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
                     }
+                    if (turns && go) {
+                        const float4 c0 = s_turn[tk + u][lane * 2], c1 = s_turn[tk + u][lane * 2 + 1];
+                        const float cs[4] = {c0.x, c0.z, c1.x, c1.z}, sn[4] = {c0.y, c0.w, c1.y, c1.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float lo = v[i], hi = v[i + 4];
+                            v[i] = lo * cs[i] - hi * sn[i];
+                            v[i + 4] = hi * cs[i] + lo * sn[i];
+                        }
+                    }
+                    out = pack8(v);
                 }
-                if (!is_v) out = pack8(v);
+                if (!go) continue;
+                const long long at = s_at[tk + u];
+                if (is_q ? at == -2 : at < 0) continue;
+                uint16_t* row = to + (is_q ? (long long)(t0 + tk + u) * a.o_stride : at);
+                *reinterpret_cast<uint2*>(row + e0) = make_uint2(out.x, out.y);
+                *reinterpret_cast<uint2*>(row + e1) = make_uint2(out.z, out.w);
             }
-            if (head >= end) continue;
-            uint16_t* to = nullptr;
-            if (is_q) to = a.q_out + (long long)t * a.o_stride + (long long)head * a.o_head;
-            else if (at >= 0) to = (is_v ? b.v + (long long)(head - a.q_heads - b.kv_heads) * b.head_stride : b.k + (long long)(head - a.q_heads) * b.head_stride) + at;
-            if (to) *reinterpret_cast<uint4*>(to + lane * 8) = out;
         }
     }
 }
 
 template <int D>
 cudaError_t launch(const AppendArgs& a, const nvfp4_device_info& dev, cudaStream_t s) {
-    constexpr int kHeads = kThreads / (D / 8);
+    constexpr int kHeads = kThreads / (D / 8), kTokens = 8;
     const int total = a.q_heads + 2 * a.b.kv_heads, steps = (total + kHeads - 1) / kHeads;
-    // Few tokens: a block for each step of a token's heads.  Many: one block per token, which shares its angles and keeps
-    // more loads in flight.
+    // Few tokens: a block for each step of a token's heads.  Many: a block for eight tokens, whose look-ups run side by side.
     const bool spread = (long long)a.b.tokens * steps <= 8LL * dev.sm_count;
-    const int per = spread ? kHeads : steps * kHeads;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(a.b.tokens, spread ? steps : 1);
+    cfg.gridDim = dim3(spread ? a.b.tokens : (a.b.tokens + kTokens - 1) / kTokens, spread ? steps : 1);
     cfg.blockDim = dim3(kThreads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -141,7 +195,7 @@ cudaError_t launch(const AppendArgs& a, const nvfp4_device_info& dev, cudaStream
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return spread ? cudaLaunchKernelEx(&cfg, kv_append_kernel<D, 1>, a, per) : cudaLaunchKernelEx(&cfg, kv_append_kernel<D, 2>, a, per);
+    return spread ? cudaLaunchKernelEx(&cfg, kv_append_kernel<D, 1, 1>, a, kHeads) : cudaLaunchKernelEx(&cfg, kv_append_kernel<D, kTokens, 4>, a, total);
 }
 
 }  // namespace

@@ -83,23 +83,10 @@ NVFP4_PAGED_HD long long place(const Batch& b, int s, int pos) {
     return (long long)page * b.page_stride + (long long)(pos - entry * b.page_size) * b.token_stride;
 }
 
-// The sequence and position of row t; false where it belongs to none or its position is negative.
-NVFP4_PAGED_HD bool find_row(const Batch& b, int t, int& seq, int& pos) {
-    int q1 = t + 1;
-    seq = t;
-    if (b.cu_q) {
-        int lo = 0, hi = b.sequences;                 // the last s with cu_q[s] <= t, by halving
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (b.cu_q[mid] <= t) lo = mid; else hi = mid;
-        }
-        seq = lo;
-        q1 = b.cu_q[lo + 1];
-        if (t < b.cu_q[lo] || t >= q1) return false;
-    } else if (t >= b.sequences) {
-        return false;
-    }
-    const long long p = (long long)b.kv_len[seq] - ((long long)q1 - t);
+// The position of row t of sequence s, [q0, q1) its rows by cu_q; false where the row is none of the sequence's or its position is negative.
+NVFP4_PAGED_HD bool row_position(const Batch& b, int s, int q0, int q1, int t, int& pos) {
+    if (t < q0 || t >= q1) return false;
+    const long long p = (long long)b.kv_len[s] - ((long long)q1 - t);
     pos = (int)p;
     return p >= 0;
 }

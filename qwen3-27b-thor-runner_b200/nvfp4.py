@@ -6,6 +6,7 @@ no CPU fallback: loading fails loudly when the CUDA library has not been built.
 """
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libnvfp4_b200.so")
@@ -151,10 +152,19 @@ def _ptr(t):
     return t.data_ptr()
 
 
+_raw_stream = None
+
+
 def _stream(stream):
     if stream is None:
-        import torch
-        return torch.cuda.current_stream().cuda_stream
+        global _raw_stream
+        if _raw_stream is None:
+            import torch
+            torch.cuda.init()
+            # the address alone, where torch gives it: building a Stream object takes 3 us of a call's 9
+            get, dev = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
+            _raw_stream = (lambda: get(dev())) if get and dev else (lambda: torch.cuda.current_stream().cuda_stream)
+        return _raw_stream()
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
@@ -189,6 +199,13 @@ class PagedBatch:
         self.c = PagedBatchStruct(_ptr(cu_q), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], sequences,
                                   sequences if tokens is None else tokens, max_q_len)
         self.address = ctypes.addressof(self.c)
+
+
+# The descriptors of the calls on a paged cache as bytes: packing them takes a third of the time that filling a ctypes structure does.
+_APPEND = struct.Struct("@6P8q4Piif4x")
+_ATTENTION = struct.Struct("@5P6qif")
+assert _APPEND.size == ctypes.sizeof(KvAppendDesc) and _ATTENTION.size == ctypes.sizeof(PagedAttentionDesc)
+_NO_ROWS = (0, 0, 0)
 
 
 def _rows(t):
@@ -316,21 +333,21 @@ class Handle:
     def kv_append(self, cache, batch, q, k, v, q_out, q_norm=None, k_norm=None, norm_eps=1e-6, inv_freq=None, positions=None, stream=None):
         """nvfp4_kv_append: norms, rotation (of 2 * len(inv_freq) elements) and append.  q, k, v and q_out are [tokens, heads, head dim] tensors
         (views with strides are fine; q and q_out None: keys and values only)."""
-        qp, qt, qh = (None, 0, 0) if q is None else _rows(q)
-        op, ot, oh = (None, 0, 0) if q is None else _rows(q_out)
+        qp, qt, qh = _NO_ROWS if q is None else _rows(q)
+        op, ot, oh = _NO_ROWS if q is None else _rows(q_out)
         kp, kt, kh = _rows(k)
         vp, vt, vh = _rows(v)
-        d = KvAppendDesc(cache.address, batch.address, qp, kp, vp, op, qt, qh, kt, kh, vt, vh, ot, oh, _ptr(q_norm), _ptr(k_norm), _ptr(inv_freq),
-                         _ptr(positions), 0 if q is None else q.shape[1], 0 if inv_freq is None else 2 * inv_freq.shape[0], norm_eps)
-        self._check(self.lib.nvfp4_kv_append(self.h, ctypes.byref(d), _stream(stream)))
+        d = _APPEND.pack(cache.address, batch.address, qp, kp, vp, op, qt, qh, kt, kh, vt, vh, ot, oh, _ptr(q_norm) or 0, _ptr(k_norm) or 0,
+                         _ptr(inv_freq) or 0, _ptr(positions) or 0, 0 if q is None else q.shape[1], 0 if inv_freq is None else 2 * inv_freq.shape[0], norm_eps)
+        self._check(self.lib.nvfp4_kv_append(self.h, d, _stream(stream)))
 
     def paged_attention(self, cache, batch, q, out, gate=None, scale=0.0, stream=None):
         """nvfp4_paged_attention: q, out and gate are [tokens, heads, head dim] tensors; scale 0 = 1 / sqrt(head dim)."""
         qp, qt, qh = _rows(q)
         op, ot, oh = _rows(out)
-        gp, gt, gh = (None, 0, 0) if gate is None else _rows(gate)
-        d = PagedAttentionDesc(cache.address, batch.address, qp, gp, op, qt, qh, gt, gh, ot, oh, q.shape[1], scale)
-        self._check(self.lib.nvfp4_paged_attention(self.h, ctypes.byref(d), _stream(stream)))
+        gp, gt, gh = _NO_ROWS if gate is None else _rows(gate)
+        d = _ATTENTION.pack(cache.address, batch.address, qp, gp, op, qt, qh, gt, gh, ot, oh, q.shape[1], scale)
+        self._check(self.lib.nvfp4_paged_attention(self.h, d, _stream(stream)))
 
     def linear_host(self, A_host, M, packed, scale, global_scale, N, K, C_host, residual_host=None, stream=None):
         self._check(self.lib.nvfp4_linear_host(self.h, _ptr(A_host), M, _ptr(packed), _ptr(scale), global_scale,

@@ -47,7 +47,12 @@ int paged_places(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int s, int
 int paged_row(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int t, int* seq, int* pos) {
     Batch x{};
     if (int e = check_batch(c, b, &x)) return e;
-    return find_row(x, t, *seq, *pos) ? 1 : 0;
+    if (!x.cu_q) {
+        *seq = t;
+        return t < x.sequences && row_position(x, t, t, t + 1, t, *pos);
+    }
+    for (*seq = x.sequences - 1; *seq > 0 && x.cu_q[*seq] > t; --*seq) {}         // the last s with cu_q[s] <= t
+    return row_position(x, *seq, x.cu_q[*seq], x.cu_q[*seq + 1], t, *pos);
 }
 int paged_sequence(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int s, int* out) {
     Batch x{};
