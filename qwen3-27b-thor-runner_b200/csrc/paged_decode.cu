@@ -145,7 +145,7 @@ struct Cursor {
     // To the next item that has units in the run [c0, c1); false behind the last one.
     __device__ __forceinline__ bool next_item(const DecodeParams& p, long long c0, long long c1, const Sequence* ahead, int base) {
         at += n.cost();
-        if (at + kItemCost >= c1) return false;
+        if (at + n.extra >= c1) return false;
         if (++item == n.items) {
             item = 0;
             do {
@@ -478,8 +478,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         const bool whole = from == 0 && at.to == at.n.chunks;
         const int rows = at.q.q_len * a.group, low_rows = rows - at.tile * kRows;
         const Row row0(a, at.q.q0, rows, at.head, at.tile * kRows + row), row1(a, at.q.q0, rows, at.head, at.tile * kRows + row + 8);
-        const int first = block_of(cost, blocks, at.at + kItemCost);
-        const int count = whole ? 1 : block_of(cost, blocks, at.at + kItemCost + at.n.chunks - 1) - first + 1;
+        const int first = block_of(cost, blocks, at.at + at.n.extra);
+        const int count = whole ? 1 : block_of(cost, blocks, at.at + at.n.extra + at.n.chunks - 1) - first + 1;
         float* part = p.parts + (size_t)part_slot(first, blockIdx.x) * kPartFloats;
         if (!whole && first == (int)blockIdx.x && tid == 0) p.split[blockIdx.x] = SplitItem{count, at.q.q0, rows, at.head, at.tile, {0, 0, 0}};
         // the i-th tile whose sum this warp writes: as the rounds go through them
@@ -661,13 +661,13 @@ paged_join_kernel(const __grid_constant__ DecodeParams p, int blocks) {
             float m[kJoinAhead / 2], l[kJoinAhead / 2], top = -INFINITY, den = 0.0f;      // part 2j + lane / 16, row lane % 16, in place j
 #pragma unroll
             for (int j = 0; j < kJoinAhead; ++j)
-                y[j] = __ldcg(reinterpret_cast<const float4*>(p.parts + (size_t)part_slot(first, first + min(j, it.count - 1)) * kPartFloats) + tile * 32 + lane);
+                y[j] = ptx::ldcg_if(j < it.count, reinterpret_cast<const float4*>(p.parts + (size_t)part_slot(first, first + j) * kPartFloats) + tile * 32 + lane);
 #pragma unroll
             for (int j = 0; j < kJoinAhead / 2; ++j) {
                 const int i = 2 * j + (lane >> 4);
-                const float* ml = p.parts + (size_t)part_slot(first, first + min(i, it.count - 1)) * kPartFloats + kRows * D + (lane & 15);
-                m[j] = i < it.count ? __ldcg(ml) : -INFINITY;
-                l[j] = i < it.count ? __ldcg(ml + kRows) : 0.0f;
+                const float* ml = p.parts + (size_t)part_slot(first, first + i) * kPartFloats + kRows * D + (lane & 15);
+                m[j] = ptx::ldcg_if(i < it.count, ml, -INFINITY);
+                l[j] = ptx::ldcg_if(i < it.count, ml + kRows, 0.0f);
                 top = fmaxf(top, m[j]);
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -709,17 +709,17 @@ paged_join_kernel(const __grid_constant__ DecodeParams p, int blocks) {
             float m[kJoinAhead / 2], l[kJoinAhead / 2];
 #pragma unroll
             for (int j = 0; j < kJoinAhead; ++j) {
-                const int i = min(i0 + j * kJoinWarps, it.count - 1);
+                const int i = i0 + j * kJoinWarps;
                 const float4* from = reinterpret_cast<const float4*>(p.parts + (size_t)part_slot(first, first + i) * kPartFloats) + tile0 * 32 + lane;
 #pragma unroll
-                for (int t = 0; t < kTiles; ++t) y[j][t] = __ldcg(from + t * 32);
+                for (int t = 0; t < kTiles; ++t) y[j][t] = ptx::ldcg_if(i < it.count, from + t * 32);
             }
 #pragma unroll
             for (int j = 0; j < kJoinAhead / 2; ++j) {
                 const int i = i0 + (2 * j + (lane >> 4)) * kJoinWarps;
-                const float* ml = p.parts + (size_t)part_slot(first, first + min(i, it.count - 1)) * kPartFloats + kRows * D + (lane & 15);
-                m[j] = i < it.count ? __ldcg(ml) : -INFINITY;
-                l[j] = i < it.count ? __ldcg(ml + kRows) : 0.0f;
+                const float* ml = p.parts + (size_t)part_slot(first, first + i) * kPartFloats + kRows * D + (lane & 15);
+                m[j] = ptx::ldcg_if(i < it.count, ml, -INFINITY);
+                l[j] = ptx::ldcg_if(i < it.count, ml + kRows, 0.0f);
             }
             float now = top;
 #pragma unroll
@@ -846,7 +846,7 @@ cudaError_t launch_paged_decode(const paged::AttentionArgs& a, int most_rows, co
     DecodeParams p{};
     p.a = a;
     p.scale_log2 = a.scale * 1.4426950408889634f;
-    p.min_cost = 3;
+    p.min_cost = item_cost(a.b.head_dim) + 1;
     p.most_rows = most_rows;
     p.piece = a.b.page_size % 16 == 0 ? 16 : a.b.page_size % 8 == 0 ? 8 : 0;
     p.split = static_cast<SplitItem*>(scratch);

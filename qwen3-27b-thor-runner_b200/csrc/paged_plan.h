@@ -95,16 +95,17 @@ NVFP4_PAGED_HD bool row_position(const Batch& b, int s, int q0, int q1, int t, i
 // tokens each.  All units in order (sequence, head, tile, chunk) are cut into equal runs, one per block.
 constexpr int kRows = 16;
 //
-// What an item costs beside its units (its rows of q, the warps' sums, the result's way out) is about kItemCost units, so that a run of
+// What an item costs beside its units (its rows of q, the warps' sums, the result's way out) is about item_cost() units, so that a run of
 // many short items would take several times as long as a run of a long one: runs are cut in places of cost, of which an item has
-// kItemCost in front of its units.  A window of more than kItemCost places holds a unit, so no run is without one.
-constexpr int kItemCost = 2;
+// item_cost() in front of its units.  A window of more than item_cost() places holds a unit, so no run is without one.  Measured: 64 sequences,
+// heads of 256, cost 2, 3, 4: 88.8, 84.4, 83.8 us; one sequence of 1501 tokens 15.5, 16.6, 17.6; 243 sequences, heads of 128: 107, 109, 117.
+NVFP4_PAGED_HD int item_cost(int head_dim) { return head_dim == 256 ? 3 : 2; }
 struct Items {
-    int tiles, items, chunks;
-    NVFP4_PAGED_HD int cost() const { return chunks + kItemCost; }              // of one item
+    int tiles, items, chunks, extra;
+    NVFP4_PAGED_HD int cost() const { return chunks + extra; }                  // of one item
 };
 NVFP4_PAGED_HD Items items_of(const Batch& b, const Sequence& q, int group, int chunk, int most_rows) {
-    Items n{0, 0, 1};
+    Items n{0, 0, 1, item_cost(b.head_dim)};
     const long long rows = (long long)q.q_len * group;
     if (rows > 0 && rows <= most_rows) {
         n.tiles = (int)((rows + kRows - 1) / kRows);
@@ -113,7 +114,7 @@ NVFP4_PAGED_HD Items items_of(const Batch& b, const Sequence& q, int group, int 
     }
     return n;
 }
-// Blocks in use: no more than there are runs of min_cost (> kItemCost) places.
+// Blocks in use: no more than there are runs of min_cost (more than an item costs beside its units) places.
 NVFP4_PAGED_HD int blocks_of(long long cost, int grid, int min_cost) { return (int)least((long long)grid, most(cost / min_cost, 1LL)); }
 NVFP4_PAGED_HD long long run_begin(long long cost, int blocks, int block) { return cost * block / blocks; }
 // The block whose run holds place c.
@@ -123,7 +124,7 @@ struct Units {
     int from, to;
 };
 NVFP4_PAGED_HD Units units_in(long long at, const Items& n, long long c0, long long c1) {
-    const long long u = at + kItemCost;
+    const long long u = at + n.extra;
     return {(int)least(most(c0 - u, 0LL), (long long)n.chunks), (int)least(most(c1 - u, 0LL), (long long)n.chunks)};
 }
 // An item that several blocks share is held in parts by blocks first .. first + count - 1: the first one's part, the only one of an item that
@@ -133,8 +134,10 @@ NVFP4_PAGED_HD int part_slot(int first, int block) { return 2 * block + (block =
 
 // ---- work of the attention of many tokens.  An item is a (sequence, tile of tile_tokens new tokens, key-value head); its units are the
 // kLongChunk keys wide chunks that its last token sees, so a prompt's tiles have more and more of them.  Items in order (sequence, tile, head) have
-// kLongCost places of cost in front of their units and are cut into runs as above.
-constexpr int kLongChunk = 128, kLongCost = 6;
+// long_cost() places of cost in front of their units and are cut into runs as above.  Measured with a cost of 2, 4, 6: a prompt of 8192 tokens, heads of
+// 256, 1098, 835, 804 us; a mixed step with heads of 128 107, 105, 112.
+constexpr int kLongChunk = 128;
+NVFP4_PAGED_HD int long_cost(int head_dim) { return head_dim == 256 ? 6 : 4; }
 
 // sum of floor((a i + b) / m) over 0 <= i < n (m > 0, a (n - 1) + b and a mod m * n + b mod m below 2^32), by swapping slope and modulus as in
 // Euclid's algorithm
@@ -156,10 +159,10 @@ NVFP4_PAGED_HD long long floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t 
 }
 
 struct LongItems {
-    int tiles, tile_tokens, heads;
+    int tiles, tile_tokens, heads, extra;
 };
 NVFP4_PAGED_HD LongItems long_items_of(const Batch& b, const Sequence& q, int group, int tile_tokens, int above_rows) {
-    LongItems n{0, tile_tokens, b.kv_heads};
+    LongItems n{0, tile_tokens, b.kv_heads, long_cost(b.head_dim)};
     if ((long long)q.q_len * group > above_rows) n.tiles = (q.q_len + tile_tokens - 1) / tile_tokens;
     return n;
 }
@@ -171,7 +174,7 @@ NVFP4_PAGED_HD int long_chunks(int limit) { return most((limit + kLongChunk - 1)
 // Places of the first `tiles` tiles of one head.
 NVFP4_PAGED_HD long long long_places(const Sequence& q, const LongItems& n, int tiles) {
     const int full = least(tiles, n.tiles - 1), step = n.tile_tokens;             // tiles whose last token is (i + 1) * step - 1
-    long long sum = (long long)tiles * kLongCost;
+    long long sum = (long long)tiles * n.extra;
     if (tiles == n.tiles && tiles > 0) sum += long_chunks(long_limit(q, n, tiles - 1));
     if (full <= 0) return sum;
     // first + (i + 1) * step keys: up to kLongChunk of them one chunk, beyond kv those that kv has

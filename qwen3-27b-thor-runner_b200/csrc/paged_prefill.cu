@@ -90,13 +90,13 @@ struct Cursor {
     __device__ __forceinline__ void set_item(long long c0, long long c1) {
         limit = long_limit(q, n, tile);
         chunks = long_chunks(limit);
-        const long long u = at + kLongCost;
+        const long long u = at + n.extra;
         chunk = (int)min(max(c0 - u, 0LL), (long long)chunks);
         to = (int)min(max(c1 - u, 0LL), (long long)chunks);
     }
     __device__ __forceinline__ bool next_item(const PrefillParams& p, long long c0, long long c1) {
-        at += chunks + kLongCost;
-        if (at + kLongCost >= c1) return false;
+        at += chunks + n.extra;
+        if (at + n.extra >= c1) return false;
         if (++head == n.heads) {
             head = 0;
             if (++tile == n.tiles) {
@@ -382,7 +382,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
         }
         const long long at = long_places(x.q, x.n, lo) * x.n.heads;
         x.tile = lo;
-        const int per = long_chunks(long_limit(x.q, x.n, lo)) + kLongCost;
+        const int per = long_chunks(long_limit(x.q, x.n, lo)) + x.n.extra;
         x.head = (int)((left - at) / per);
         x.at = c0 - (left - at) + (long long)x.head * per;
         x.set_item(c0, c1);
@@ -623,9 +623,9 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
         while (more) {
             const int n = at.to - at.chunk, live = at.live(p);
             const bool whole = at.chunk == 0 && at.to == at.chunks;
-            const int first = whole ? id : block_of(cost, pairs, at.at + kLongCost);
+            const int first = whole ? id : block_of(cost, pairs, at.at + at.n.extra);
             if (!whole && first == id && rank == 0 && tid == 96)
-                p.split[id] = LongSplit{block_of(cost, pairs, at.at + kLongCost + at.chunks - 1) - first + 1, at.q.q0, at.q.q_len, at.tile, at.head, {0, 0, 0}};
+                p.split[id] = LongSplit{block_of(cost, pairs, at.at + at.n.extra + at.chunks - 1) - first + 1, at.q.q0, at.q.q_len, at.tile, at.head, {0, 0, 0}};
             int see[F::kNT];
             bool there[F::kNT];
             float m[F::kNT], l[F::kNT];
@@ -865,13 +865,14 @@ paged_prefill_join_kernel(const __grid_constant__ PrefillParams p, int pairs) {
             float m[kJoinAhead], l[kJoinAhead];
 #pragma unroll
             for (int j = 0; j < kJoinAhead; ++j) {
-                const float* part = p.parts + (size_t)(part_slot(first, first + min(i0 + j, it.count - 1)) * 2 + (tile & 1)) * kMaxPartFloats;
+                const bool is = i0 + j < it.count;
+                const float* part = p.parts + (size_t)(part_slot(first, first + i0 + j) * 2 + (tile & 1)) * kMaxPartFloats;
                 const float* ml = part + F::kNT * kTile * D + (tile >> 1) * (2 * kTile) + row;
                 const float4* from = reinterpret_cast<const float4*>(part) + ((tile >> 1) * (D / 4) + c0 / 4) * kTile + row;
-                y[j][0] = __ldcg(from);
-                y[j][1] = __ldcg(from + kTile);
-                m[j] = __ldcg(ml);
-                l[j] = __ldcg(ml + kTile);
+                y[j][0] = ptx::ldcg_if(is, from);
+                y[j][1] = ptx::ldcg_if(is, from + kTile);
+                m[j] = ptx::ldcg_if(is, ml, -INFINITY);
+                l[j] = ptx::ldcg_if(is, ml + kTile, 0.0f);
             }
             float now = top;
 #pragma unroll
@@ -977,7 +978,7 @@ bool launch_paged_prefill(const paged::AttentionArgs& a, int above_rows, const n
     p.a = a;
     p.scale_log2 = a.scale * 1.4426950408889634f;
     p.above_rows = above_rows;
-    p.min_cost = kLongCost + 1;
+    p.min_cost = long_cost(a.b.head_dim) + 1;
     p.split = static_cast<LongSplit*>(scratch);
     p.parts = reinterpret_cast<float*>(static_cast<char*>(scratch) + kSplitBytes);
     const bool done = a.b.head_dim == 64 ? launch<64>(p, dev, s, e) : a.b.head_dim == 128 ? launch<128>(p, dev, s, e) : launch<256>(p, dev, s, e);

@@ -295,6 +295,21 @@ __device__ __forceinline__ uint2 ld_volatile_v2(const void* p) {
     return v;
 }
 
+// Loads past L1 of what may not be there (zero then), under a predicate and not behind a branch: a run of them goes out together.
+__device__ __forceinline__ float4 ldcg_if(bool there, const float4* p) {
+    float4 v;
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %5, 0;\n\tmov.f32 %0, 0f00000000;\n\tmov.f32 %1, 0f00000000;\n\tmov.f32 %2, 0f00000000;\n\tmov.f32 %3, 0f00000000;\n\t"
+        "@q ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "=&f"(v.x), "=&f"(v.y), "=&f"(v.z), "=&f"(v.w) : "l"(p), "r"((uint32_t)there) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ldcg_if(bool there, const float* p, float otherwise) {
+    float v;
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %3, 0;\n\tmov.f32 %0, %2;\n\t@q ld.global.cg.f32 %0, [%1];\n\t}" : "=&f"(v) : "l"(p), "f"(otherwise), "r"((uint32_t)there) : "memory");
+    return v;
+}
+
 // Sixteen bytes as one access (relaxed, GPU scope): the words arrive together.
 __device__ __forceinline__ void st_relaxed_b128(void* p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile(

@@ -79,7 +79,7 @@ int paged_long_places(int q_len, int kv_len, int max_kv, int tile_tokens) {
     for (int t = 0; t < n.tiles; ++t) {
         const int limit = long_limit(q, n, t);
         if (limit < 0 || limit > q.kv) return -1;
-        sum += long_chunks(limit) + kLongCost;
+        sum += long_chunks(limit) + long_cost(x.head_dim);
         bad += long_places(q, n, t + 1) != sum;
     }
     return bad;
@@ -109,7 +109,7 @@ int paged_walk(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int group, i
     std::vector<int> held(blocks, 0), slots(2 * blocks, 0);
     for (size_t i = 0; i < at.size(); ++i) {
         const Items& n = items[i];
-        const int first = block_of(cost, blocks, at[i] + kItemCost), last = block_of(cost, blocks, at[i] + kItemCost + n.chunks - 1);
+        const int first = block_of(cost, blocks, at[i] + n.extra), last = block_of(cost, blocks, at[i] + n.extra + n.chunks - 1);
         if (first < 0 || last >= blocks || last < first) return 4;
         int next = 0;
         for (int k = first > 0 ? first - 1 : 0; k <= last + 1 && k < blocks; ++k) {
