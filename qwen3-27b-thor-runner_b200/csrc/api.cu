@@ -785,10 +785,12 @@ int nvfp4_paged_attention(nvfp4_handle* h, const nvfp4_paged_attention_desc* d, 
     a.b.status = reinterpret_cast<unsigned int*>(h->workspace);
     OnDevice on(h->dev.device);
     if (on.e != cudaSuccess) return (int)on.e;
-    // Up to 16 rows (new tokens x heads of a group) of a sequence share one tile of the few-token kernel, which runs at the rate of the
-    // cache's bytes; a tcgen05 tile holds 128.  The host knows bounds only: where they leave no room for sequences of both kinds, one kernel
-    // takes all, otherwise each takes its own.
-    constexpr int kFewRows = paged::kRows;
+    // 16 rows (new tokens x heads of a group) of a sequence share a tile of the few-token kernel, which runs at the rate of the cache's bytes, read once for
+    // each tile; a tcgen05 tile holds 128, and a pair of SMs two to four.  Measured, few-token kernel and the other, us: 32 sequences of 8 tokens x 4 heads of
+    // 128 (32 rows) 131, 199; 24 of 4 x 8 of 64 (32) 31, 54; 12 of 4 x 6 of 256 (24) 41, 41; 64 of those 178, 163; 16 of 8 x 6 of 256 (48) 86, 67; 32 of
+    // 16 x 4 of 128 (64) 242, 199.  Two tiles it is.  The host knows bounds only: where they leave no room for sequences of both kinds, one kernel takes all,
+    // otherwise each takes its own.
+    constexpr int kFewRows = 2 * paged::kRows;
     cudaError_t e = cudaSuccess;
     int nl = 0;
     bool all = true;                 // the few-token kernel takes every sequence
