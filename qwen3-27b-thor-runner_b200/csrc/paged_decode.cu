@@ -294,7 +294,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                 ok &= 0xFFFFu;
                 if (lane == 0) s_ok[warp * F::kStages + stage] = ok;
                 const long long off = there ? (long long)page_ahead * b.page_stride + (long long)slot_ahead * b.token_stride + (long long)ld.head * b.head_stride + col0 : 0;
-                if (ok) {
+                if (tok0 < ld.limit) {                       // no page at all: zeros too, the values are multiplied
                     constexpr int kPer = F::kWidth / 8;      // 16-byte pieces of a token
 #pragma unroll
                     for (int i = 0; i < kGroup * kPer / 32; ++i) {

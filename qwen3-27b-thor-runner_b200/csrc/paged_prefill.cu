@@ -230,19 +230,19 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return d;
 }
 
-__device__ __forceinline__ float min_nan(float x, float y) {             // NaN stays NaN
-    float d;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(x), "f"(y));
-    return d;
+__device__ __forceinline__ float reciprocal(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 // Two values times the sigmoids of their BF16 gates, 1 / (1 + u) with u = 2^(-log2(e) gate).  2^x and 1 / x come from the same unit, four values a clock and
-// scheduler, which would be all that a tile's way out waits for: one reciprocal, of (1 + u) (1 + v), serves both.  u stays below 2^63 for that: a gate
-// below -43.6 counts as -43.6, a factor of 1e-19.
+// scheduler, which would be all that a tile's way out waits for: one reciprocal, of (1 + u) (1 + v), serves both where the product stays in range (gates
+// above -43.6).
 __device__ __forceinline__ uint32_t gated(float x, float y, uint32_t gate) {
     const float c = -1.4426950408889634f;
-    const float u = 1.0f + min_nan(ex2(__uint_as_float(gate << 16) * c), 0x1p63f), v = 1.0f + min_nan(ex2(__uint_as_float(gate & 0xFFFF0000u) * c), 0x1p63f);
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(u * v));
+    const float u = 1.0f + ex2(__uint_as_float(gate << 16) * c), v = 1.0f + ex2(__uint_as_float(gate & 0xFFFF0000u) * c);
+    if (!(u <= 0x1p63f && v <= 0x1p63f)) return pack_bf16(x * reciprocal(u), y * reciprocal(v));           // NaN goes here, too
+    const float r = reciprocal(u * v);
     return pack_bf16(x * (v * r), y * (u * r));
 }
 // 16 rows and 32 columns: register 4 i + 2 h + e of a lane is row lane / 4 + 8 h, column 8 i + 2 (lane % 4) + e.
@@ -876,8 +876,7 @@ paged_prefill_join_kernel(const __grid_constant__ PrefillParams p, int pairs) {
             }
             float now = top;
 #pragma unroll
-            for (int j = 0; j < kJoinAhead; ++j)
-                if (i0 + j < it.count) now = fmaxf(now, m[j]);
+            for (int j = 0; j < kJoinAhead; ++j) now = fmaxf(now, m[j]);
             const float back = top == -INFINITY ? 0.0f : ex2(top - now);
             top = now;
             den *= back;
@@ -885,8 +884,7 @@ paged_prefill_join_kernel(const __grid_constant__ PrefillParams p, int pairs) {
             for (int e = 0; e < 8; ++e) x[e] *= back;
 #pragma unroll
             for (int j = 0; j < kJoinAhead; ++j) {
-                if (i0 + j >= it.count || m[j] == -INFINITY) continue;
-                const float w = ex2(m[j] - now);
+                const float w = m[j] == -INFINITY ? 0.0f : ex2(m[j] - now);         // a sum of NaN stays one
                 den += w * l[j];
                 x[0] = fmaf(y[j][0].x, w, x[0]); x[1] = fmaf(y[j][0].y, w, x[1]); x[2] = fmaf(y[j][0].z, w, x[2]); x[3] = fmaf(y[j][0].w, w, x[3]);
                 x[4] = fmaf(y[j][1].x, w, x[4]); x[5] = fmaf(y[j][1].y, w, x[5]); x[6] = fmaf(y[j][1].z, w, x[6]); x[7] = fmaf(y[j][1].w, w, x[7]);
@@ -970,8 +968,9 @@ cudaError_t configure_paged_prefill() {
     return e;
 }
 
-// Whole boxes of 16 tokens, a group of heads that fits a tile, a maximum that grows with the products.
-bool paged_prefill_supported(const paged::AttentionArgs& a) { return a.b.page_size % 16 == 0 && a.group <= kTile && a.scale > 0.0f; }
+// Whole boxes of 16 tokens, a group of heads that fits a tile, a maximum that grows with the products (and a scale that is none of the numbers
+// taken for zero, which would make NaN of a hidden score).
+bool paged_prefill_supported(const paged::AttentionArgs& a) { return a.b.page_size % 16 == 0 && a.group <= kTile && a.scale >= 1e-30f; }
 
 bool launch_paged_prefill(const paged::AttentionArgs& a, int above_rows, const nvfp4_device_info& dev, void* scratch, int* launches, cudaStream_t s, cudaError_t* e) {
     PrefillParams p{};

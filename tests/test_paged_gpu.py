@@ -369,3 +369,155 @@ def test_launches_are_counted(handle):
     before = handle.launch_count()
     handle.paged_attention(cache, batch, c.q, c.out)       # no rows: nothing to do
     assert handle.launch_count() == before
+
+
+# ---------------------------------------------------------------- what no ordinary batch brings together
+
+FEW_AND_MANY = [[1] * 6, [1, 3, 4, 2], [90, 1, 260], [33]]      # new tokens: either kernel, and both
+
+
+@pytest.mark.parametrize("dim,q_heads,kv_heads", [(256, 12, 2), (128, 16, 4), (64, 6, 2)])
+@pytest.mark.parametrize("new", FEW_AND_MANY)
+def test_gates_of_any_size(handle, dim, q_heads, kv_heads, new):
+    """Far beyond what the exponential holds, in either direction, beside ordinary ones: -inf closes, inf opens."""
+    c = ref.Case(new, [3000] + [40] * (len(new) - 1), q_heads, kv_heads, dim, 16, seed=dim + len(new), gate=True)
+    g = torch.Generator().manual_seed(3)
+    far = torch.tensor([-float("inf"), float("inf"), -43.5, -43.75, -60.0, -87.0, -120.0, -3e38, 60.0, 3e38]).to(torch.bfloat16)
+    pick = torch.randint(0, 4 * len(far), c.gate.shape, generator=g)
+    c.gate = torch.where(pick.cuda() < len(far), far.cuda()[pick.cuda() % len(far)], c.gate)
+    check_attention(handle, c)
+
+
+@pytest.mark.parametrize("dim,q_heads,kv_heads", [(256, 12, 2), (128, 16, 4), (64, 6, 2)])
+@pytest.mark.parametrize("new", FEW_AND_MANY)
+def test_nan_stays_with_its_query_and_its_gate(handle, dim, q_heads, kv_heads, new):
+    c = ref.Case(new, [9000] + [40] * (len(new) - 1), q_heads, kv_heads, dim, 16, seed=dim + len(new), gate=True)
+    want, tol = ref.attention(c)
+    row, r2 = c.rows // 2, c.rows - 1
+    c.q[row, 1, 5] = c.q[0, q_heads - 1, 0] = float("nan")
+    c.gate[r2, 0, 3] = c.gate[r2, 2, 8] = float("nan")
+    nan = torch.zeros_like(tol, dtype=torch.bool)
+    nan[row, 1] = nan[0, q_heads - 1] = nan[r2, 0, 3] = nan[r2, 2, 8] = True
+    cache, batch = c.objects(nvfp4)
+    handle.paged_attention(cache, batch, c.q, c.out, gate=c.gate)
+    torch.cuda.synchronize()
+    assert torch.equal(torch.isnan(c.out), nan)
+    assert ref.worst(torch.where(nan, 0, c.out), torch.where(nan, 0, want), tol) <= 1.0
+
+
+@pytest.mark.parametrize("page", [1, 4, 8, 12, 16, 64])
+@pytest.mark.parametrize("dim,q_heads,kv_heads", [(256, 6, 1), (128, 4, 2), (64, 3, 3)])
+@pytest.mark.parametrize("new", [1, 2, 40])
+def test_whole_units_without_a_page_behind_values_of_nan(page, dim, q_heads, kv_heads, new):
+    """Every second sequence has values of NaN, which stay behind in shared memory; the others lack pages for more tokens than a unit holds, in
+    front, in the middle and at the end.  Theirs is the attention over the pages that are there."""
+    h = nvfp4.Handle(0, 16 << 20)
+    n, length = 120 if new < 40 else 12, 400
+    c = ref.Case([new] * n, [length - new] * n, q_heads, kv_heads, dim, page, seed=page)
+    gone = torch.zeros(length, dtype=torch.bool)
+    for s in range(n):
+        if s % 2 == 0:
+            c.v_cache[c.table[s].long().cuda()] = float("nan")
+            continue
+        first = [0, 96, 208][s // 2 % 3]
+        entries = range(-(-first // page), -(-first // page) + 192 // page)
+        for e in entries:
+            c.table_dev[s, e] = [-1, c.num_pages][e % 2]
+    cache, batch = c.objects(nvfp4)
+    h.paged_attention(cache, batch, c.q, c.out)
+    torch.cuda.synchronize()
+    out = c.out.view(n, new, q_heads, dim)
+    assert bool(torch.isnan(out[0::2]).all()) and bool(torch.isfinite(out[1::2]).all())
+    assert h.device_status() == 0xA01
+    g = q_heads // kv_heads
+    for s in (1, 3, 5, n - 1):
+        there = ((c.table_dev[s] >= 0) & (c.table_dev[s] < c.num_pages)).repeat_interleave(page)[:length]
+        k, v = c.keys(c.k_cache, s, length).cuda(), c.keys(c.v_cache, s, length).cuda()
+        seen = there[None, :] & (torch.arange(length, device="cuda")[None, :] <= torch.arange(length - new, length, device="cuda")[:, None])
+        for hd in range(q_heads):
+            t = (c.q[s * new:(s + 1) * new, hd].double() @ k[:, hd // g].T * dim ** -0.5).masked_fill(~seen, -float("inf"))
+            w = torch.softmax(t, -1)
+            want, size = w @ v[:, hd // g], w @ v[:, hd // g].abs()
+            tol = 2 * ref.BF16_HALF_STEP * size + 1e-5 * size + ref.BF16_HALF_STEP * want.abs() + 1e-30
+            assert ref.worst(out[s, :, hd], want, tol) <= 1.0
+    h.close()
+
+
+@pytest.mark.parametrize("dim,q_heads,kv_heads,new", [(256, 12, 2, 11), (256, 2, 2, 40), (128, 16, 4, 40), (128, 8, 8, 5), (64, 6, 1, 300), (64, 4, 2, 17)])
+def test_few_tokens_behind_a_very_long_past(handle, dim, q_heads, kv_heads, new):
+    """An item whose parts are more than a join has under way at once."""
+    c = ref.Case([new], [30011], q_heads, kv_heads, dim, 64, seed=dim + new, gate=dim == 256)
+    check_attention(handle, c, times=2)
+
+
+@pytest.mark.parametrize("dim,q_heads,kv_heads", [(256, 24, 2), (128, 32, 8), (64, 40, 2)])
+def test_rows_around_the_border_of_the_two_kernels(handle, dim, q_heads, kv_heads):
+    """Sequences of one to forty rows in one call, each by the kernel for its own."""
+    new = [1, 2, 3, 4, 5, 7, 8, 9, 16, 17, 1, 32, 33, 40]
+    c = ref.Case(new, [(i * 977) % 3000 for i in range(len(new))], q_heads, kv_heads, dim, 16, seed=dim, pad=3, lead=2, gate=True)
+    check_attention(handle, c)
+
+
+@pytest.mark.parametrize("hint", [1, 2, 50, 100000])
+def test_the_longest_run_may_be_guessed_wrong(handle, hint):
+    c = ref.Case([70, 1, 30, 2], [100, 900, 0, 33], 8, 2, 128, 16, seed=hint, pad=5)
+    cache, _ = c.objects(nvfp4)
+    want, tol = ref.attention(c)
+    handle.paged_attention(cache, nvfp4.PagedBatch(c.kv_dev, c.table_dev, tokens=c.rows, cu_q=c.cu_dev, max_q_len=hint), c.q, c.out)
+    torch.cuda.synchronize()
+    assert ref.worst(c.out, want, tol) <= 1.0
+
+
+def test_more_heads_in_a_group_than_a_tile_has_rows(handle):
+    c = ref.Case([3, 1, 40], [50, 700, 9], 130, 1, 64, 16, seed=4)
+    check_attention(handle, c)
+    c = ref.Case([3, 1, 40], [50, 700, 9], 128, 1, 128, 16, seed=5, gate=True)
+    check_attention(handle, c)
+
+
+@pytest.mark.parametrize("new", [1, 60])
+def test_sequences_that_share_a_prefix(handle, new):
+    c = ref.Case([new] * 5, [512] * 5, 8, 2, 128, 32, seed=6)
+    c.table[1:, :16] = c.table[0, :16]
+    c.table_dev = c.table.cuda()
+    check_attention(handle, c)
+
+
+def test_two_handles_on_two_streams_at_once():
+    handles = [nvfp4.Handle(0, 16 << 20) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    cases = [ref.Case([200, 1, 3], [4000, 9000, 50], 12, 2, 256, 16, seed=s, gate=True) for s in (1, 2)]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for h, s, c in zip(handles, streams, cases):
+            with torch.cuda.stream(s):
+                h.paged_attention(*c.objects(nvfp4), c.q, c.out, gate=c.gate)
+    torch.cuda.synchronize()
+    for h, c in zip(handles, cases):
+        want, tol = ref.attention(c)
+        assert ref.worst(c.out, want, tol) <= 1.0 and h.device_status() == 0
+        h.close()
+
+
+def test_calls_behind_one_another_share_the_scratch(handle):
+    """Different batches, kernels and head sizes through one handle without a wait in between."""
+    cases = [ref.Case(n, p, q, k, d, 16, seed=i) for i, (n, p, q, k, d) in enumerate([
+        ([1], [20000], 12, 2, 256), ([300], [5000], 8, 2, 128), ([1] * 40, [700] * 40, 4, 4, 64), ([500, 1], [0, 9000], 6, 1, 256), ([1] * 3, [5000] * 3, 16, 2, 128)])]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for c in cases:
+            handle.paged_attention(*c.objects(nvfp4), c.q, c.out)
+    torch.cuda.synchronize()
+    for c in cases:
+        want, tol = ref.attention(c)
+        assert ref.worst(c.out, want, tol) <= 1.0
+
+
+def test_nothing_to_do(handle):
+    c = ref.Case([0, 0], [5, 9], 4, 2, 128, 16, seed=1, pad=4)
+    cache, batch = c.objects(nvfp4)
+    handle.paged_attention(cache, batch, c.q, c.out)
+    k = c.k_cache.clone()
+    handle.kv_append(cache, batch, c.q, c.k, c.v, c.out)
+    torch.cuda.synchronize()
+    assert bool((c.out == 7).all()) and torch.equal(c.k_cache, k)
