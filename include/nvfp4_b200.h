@@ -60,7 +60,8 @@ typedef struct nvfp4_quantized_weight {
  * Replaces the reference's process-global state (lazy dequant scratch and
  * cuBLAS handles, src/engine/dense_gemm_fp4_sm110.cu:428,470-486) and its
  * init_fp4_cublaslt()/cleanup_fp4_cublaslt() hooks (:430-441): one handle per
- * device, workspace sized once at creation. */
+ * device, workspace sized once at creation.  Beside the workspace a handle allocates
+ * 44 MB for nvfp4_paged_attention, so that no call allocates. */
 int nvfp4_create(int device, size_t workspace_bytes, nvfp4_handle** out);
 int nvfp4_destroy(nvfp4_handle* h);
 /* Workspace needed so that every call with M<=max_M, N<=max_N, K<=max_K succeeds.  For max_M <= 16 it leaves out
@@ -441,7 +442,8 @@ int nvfp4_linear_host(nvfp4_handle* h, const void* A_host, int M,
 /* Reads the sticky device-side status word of the handle (synchronises the device).
  * 0 = no kernel of this handle ever gave up a bounded wait; otherwise the code of the first
  * wait that ran out (0x1xx producer ring slot, 0x2xx consumer ring slot, 0x300 cross-CTA
- * partial flag, 0x4xx tensor-core pipeline). */
+ * partial flag, 0x4xx tensor-core pipeline, 0xA10 a ring slot and 0xA2x to 0xA4x the pipeline of
+ * nvfp4_paged_attention), or 0xA01: a place out of bounds in a paged cache was left out. */
 int nvfp4_device_status(nvfp4_handle* h, unsigned int* status);
 
 /* Number of kernels this library has launched on the handle since creation. */

@@ -33,7 +33,7 @@ struct nvfp4_handle {
     int fp4_stream_min_m = 10;                   // from this token count on its activations travel through the ring (decode_fp4_stream.cu)
     int gemm_weight_rounding = 0;                // above 8 tokens: the reference's BF16-rounded weights (its GEMM branch)
     unsigned long long launches = 0;
-    char* paged_scratch = nullptr;               // parts and counters of split sequences in nvfp4_paged_attention
+    char* paged_scratch = nullptr;               // parts of split sequences in nvfp4_paged_attention (44 MB on 148 SMs)
     int host_direct_out = 1;                     // nvfp4_linear_host: kernels store into a pinned, device-mapped C_host themselves
     // scale tensors in which nvfp4_scan_scales found a byte 0x7F / 0xFF: the tensor core reads those as NaN, so
     // these weights stay on the kernels that decode the scale themselves
@@ -787,8 +787,8 @@ int nvfp4_paged_attention(nvfp4_handle* h, const nvfp4_paged_attention_desc* d, 
     if (on.e != cudaSuccess) return (int)on.e;
     // 16 rows (new tokens x heads of a group) of a sequence share a tile of the few-token kernel, which runs at the rate of the cache's bytes, read once for
     // each tile; a tcgen05 tile holds 128, and a pair of SMs two to four.  Measured, few-token kernel and the other, us: 32 sequences of 8 tokens x 4 heads of
-    // 128 (32 rows) 131, 199; 24 of 4 x 8 of 64 (32) 31, 54; 12 of 4 x 6 of 256 (24) 41, 41; 64 of those 178, 163; 16 of 8 x 6 of 256 (48) 86, 67; 32 of
-    // 16 x 4 of 128 (64) 242, 199.  Two tiles it is.  The host knows bounds only: where they leave no room for sequences of both kinds, one kernel takes all,
+    // 128 (32 rows) 131, 199; 24 of 4 x 8 of 64 (32) 31, 54; 64 of 4 x 6 of 256 (24) 178, 163; 16 of 8 x 6 of 256 (48) 86, 67; 12 of 4 x 12 of 256 (48)
+    // 42, 41; 32 of 16 x 4 of 128 (64) 242, 199.  Two tiles it is.  The host knows bounds only: where they leave no room for sequences of both kinds, one kernel takes all,
     // otherwise each takes its own.
     constexpr int kFewRows = 2 * paged::kRows;
     cudaError_t e = cudaSuccess;

@@ -208,7 +208,7 @@ cudaError_t configure_skinny_umma();
 cudaError_t launch_skinny_umma(const LinearArgs& a, nvfp4_device_info& dev, void* scratch, size_t scratch_bytes,
                                size_t offset, int* launches, cudaStream_t s);
 
-// --- the paged cache (paged_plan.h has the calls' arguments): kv_append.cu, paged_decode.cu.
+// --- the paged cache (paged_plan.h has the calls' arguments): kv_append.cu, paged_decode.cu, paged_prefill.cu.
 cudaError_t launch_kv_append(const paged::AppendArgs& a, const nvfp4_device_info& dev, int* launches, cudaStream_t s);
 // The attention's own scratch: the parts of split items.
 size_t paged_scratch_bytes(int sm_count);

@@ -21,6 +21,11 @@
 // Work is shared as in the attention of few tokens: units of all (sequence, tiles, head) items in order, a prompt's later tiles with more of
 // them, cut into equal runs, one persistent pair of blocks per pair of SMs; parts of split items (FP32 results, maxima, sums) are added by a second kernel.
 // Keys behind the item's last one and those of pages out of bounds are masked, and their values zeroed in shared memory, whatever lies there.
+//
+// Measured: a chunk of 256 tokens behind 16384 (24 heads over 2 of 256) 99 us, 1.05 PFLOP/s; a prompt of 8192 705-800 us by the clock the power leaves, 1.03 to
+// 1.17; 149 tokens 18 us, of which the products are 1.  A unit takes 2600 clocks with heads of 256 (products 2 x 1024, but the first one waits for shared memory,
+// 1500, and the second for tensor memory's operand, 1490; the weights 1900, over two buffers), 4200 for four tiles of 128; an item several thousand for
+// its way out (results from tensor memory, gates, rows written), which only the next item's loads and first scores overlap.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
