@@ -176,12 +176,14 @@ class KvCache:
 
     def __init__(self, k, v, order="token"):
         token, head = (1, 2) if order == "token" else (2, 1)
-        if order not in ("token", "head") or k.shape != v.shape or k.stride() != v.stride() or k.dim() != 4 or k.stride(3) != 1:
-            raise ValueError("k and v: 4-D tensors of the same shape and strides, the head's values dense; order 'token' or 'head'")
+        if order not in ("token", "head") or k.shape != v.shape or k.stride() != v.stride() or k.dim() != 4 or k.stride(3) != 1 or \
+                any(t.element_size() != 2 or not t.is_floating_point() for t in (k, v)):
+            raise ValueError("k and v: 4-D BF16 tensors of the same shape and strides, the head's values dense; order 'token' or 'head'")
         self.keep = (k, v)
         self.c = KvCacheStruct(k.data_ptr(), v.data_ptr(), k.shape[0], k.shape[token], k.shape[head], k.shape[3],
                                k.stride(0), k.stride(token), k.stride(head))
         self.address = ctypes.addressof(self.c)
+        self.heads, self.dim = k.shape[head], k.shape[3]
 
 
 class PagedBatch:
@@ -199,21 +201,23 @@ class PagedBatch:
         self.c = PagedBatchStruct(_ptr(cu_q), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], sequences,
                                   sequences if tokens is None else tokens, max_q_len)
         self.address = ctypes.addressof(self.c)
+        self.tokens = self.c.tokens
 
 
 # The descriptors of the calls on a paged cache as bytes: packing them takes a third of the time that filling a ctypes structure does.
 _APPEND = struct.Struct("@6P8q4Piif4x")
 _ATTENTION = struct.Struct("@5P6qif")
 assert _APPEND.size == ctypes.sizeof(KvAppendDesc) and _ATTENTION.size == ctypes.sizeof(PagedAttentionDesc)
-_NO_ROWS = (0, 0, 0)
+_NO_ROWS = (0, 0, 0, 0)
 
 
-def _rows(t):
-    """Address, token stride and head stride of a [tokens, heads, head dim] tensor."""
+def _rows(t, tokens, dim):
+    """Address, token stride, head stride and heads of a [tokens, heads, head dim] tensor."""
+    n, heads, d = t.shape
     a, b, c = t.stride()
-    if c != 1 or a == 0 or b == 0:       # 0 would mean dense
-        raise ValueError("a [tokens, heads, head dim] tensor whose heads are dense and that repeats nothing")
-    return t.data_ptr(), a, b
+    if c != 1 or a == 0 or b == 0 or n < tokens or d != dim:       # a stride of 0 would mean dense
+        raise ValueError("a [tokens, heads, head dim] tensor with the batch's tokens and the cache's head dim, whose heads are dense and that repeats nothing")
+    return t.data_ptr(), a, b, heads
 
 
 class Handle:
@@ -333,20 +337,27 @@ class Handle:
     def kv_append(self, cache, batch, q, k, v, q_out, q_norm=None, k_norm=None, norm_eps=1e-6, inv_freq=None, positions=None, stream=None):
         """nvfp4_kv_append: norms, rotation (of 2 * len(inv_freq) elements) and append.  q, k, v and q_out are [tokens, heads, head dim] tensors
         (views with strides are fine; q and q_out None: keys and values only)."""
-        qp, qt, qh = _NO_ROWS if q is None else _rows(q)
-        op, ot, oh = _NO_ROWS if q is None else _rows(q_out)
-        kp, kt, kh = _rows(k)
-        vp, vt, vh = _rows(v)
-        d = _APPEND.pack(cache.address, batch.address, qp, kp, vp, op, qt, qh, kt, kh, vt, vh, ot, oh, _ptr(q_norm) or 0, _ptr(k_norm) or 0,
-                         _ptr(inv_freq) or 0, _ptr(positions) or 0, 0 if q is None else q.shape[1], 0 if inv_freq is None else 2 * inv_freq.shape[0], norm_eps)
+        tokens, dim = batch.tokens, cache.dim
+        qp, qt, qh, heads = _NO_ROWS if q is None else _rows(q, tokens, dim)
+        op, ot, oh, out_heads = _NO_ROWS if q is None else _rows(q_out, tokens, dim)
+        kp, kt, kh, k_heads = _rows(k, tokens, dim)
+        vp, vt, vh, v_heads = _rows(v, tokens, dim)
+        if heads != out_heads or k_heads != cache.heads or v_heads != cache.heads:
+            raise ValueError("q and q_out have the same heads, k and v the cache's")
+        d = _APPEND.pack(cache.address, batch.address, qp, kp, vp, op, qt, qh, kt, kh, vt, vh, ot, oh, 0 if q_norm is None else q_norm.data_ptr(),
+                         0 if k_norm is None else k_norm.data_ptr(), 0 if inv_freq is None else inv_freq.data_ptr(), 0 if positions is None else positions.data_ptr(),
+                         heads, 0 if inv_freq is None else 2 * inv_freq.numel(), norm_eps)
         self._check(self.lib.nvfp4_kv_append(self.h, d, _stream(stream)))
 
     def paged_attention(self, cache, batch, q, out, gate=None, scale=0.0, stream=None):
         """nvfp4_paged_attention: q, out and gate are [tokens, heads, head dim] tensors; scale 0 = 1 / sqrt(head dim)."""
-        qp, qt, qh = _rows(q)
-        op, ot, oh = _rows(out)
-        gp, gt, gh = _NO_ROWS if gate is None else _rows(gate)
-        d = _ATTENTION.pack(cache.address, batch.address, qp, gp, op, qt, qh, gt, gh, ot, oh, q.shape[1], scale)
+        tokens, dim = batch.tokens, cache.dim
+        qp, qt, qh, heads = _rows(q, tokens, dim)
+        op, ot, oh, out_heads = _rows(out, tokens, dim)
+        gp, gt, gh, gate_heads = (0, 0, 0, heads) if gate is None else _rows(gate, tokens, dim)
+        if not heads == out_heads == gate_heads:
+            raise ValueError("q, out and gate have the same heads")
+        d = _ATTENTION.pack(cache.address, batch.address, qp, gp, op, qt, qh, gt, gh, ot, oh, heads, scale)
         self._check(self.lib.nvfp4_paged_attention(self.h, d, _stream(stream)))
 
     def linear_host(self, A_host, M, packed, scale, global_scale, N, K, C_host, residual_host=None, stream=None):

@@ -221,3 +221,30 @@ def test_places_of_causal_tiles(lib):
         max_kv = rng.choice([2147418111, rng.randint(1, 400), rng.randint(1, 20000)])
         step = rng.choice([1, 2, 10, 21, 32, 128, 256, rng.randint(1, 256)])
         assert lib.paged_long_places(q, kv, max_kv, step) == 0, (q, kv, max_kv, step)
+
+
+def test_the_binding_refuses_tensors_that_do_not_fit():
+    """What the pointers cannot tell the library.  No call reaches it."""
+    torch = pytest.importorskip("torch")
+    h = object.__new__(nvfp4.Handle)                    # without a device: every call below ends in front of the library
+    h.h, h.lib = None, None
+    new = lambda *s, dtype=torch.bfloat16: torch.zeros(s, dtype=dtype)
+    k = new(4, 16, 2, 64)
+    cache = nvfp4.KvCache(k, k.clone())
+    kv, table = torch.ones(3, dtype=torch.int32), torch.zeros(3, 2, dtype=torch.int32)
+    batch = nvfp4.PagedBatch(kv, table)
+    q, kn = new(3, 6, 64), new(3, 2, 64)
+    for args in [(q, new(3, 1, 64), kn, q.clone()), (q, kn, new(3, 4, 64), q.clone()), (q, kn, new(3, 2, 32), q.clone()), (q, new(2, 2, 64), kn, q.clone()), (q, kn, kn, new(3, 4, 64)),
+                 (new(3, 6, 32), kn, kn, new(3, 6, 32)), (new(2, 6, 64), kn, kn, q), (q, kn, new(1, 2, 64).expand(3, 2, 64), q.clone()),
+                 (q, kn, new(3, 2, 128)[..., ::2], q.clone())]:
+        with pytest.raises(ValueError):
+            h.kv_append(cache, batch, *args)
+    for args, kw in [((q, new(3, 4, 64)), {}), ((q, new(2, 6, 64)), {}), ((q, q.clone()), {"gate": new(3, 5, 64)}), ((new(3, 6, 32), new(3, 6, 32)), {}), ((new(3, 6, 128), new(3, 6, 128)), {}),
+                     ((q, q.clone()), {"gate": new(3, 6, 32)})]:
+        with pytest.raises(ValueError):
+            h.paged_attention(cache, batch, *args, **kw)
+    for bad in [lambda: nvfp4.KvCache(k, new(4, 16, 2, 128)), lambda: nvfp4.KvCache(k.float(), k.float()), lambda: nvfp4.KvCache(k, k, order="page"),
+                lambda: nvfp4.KvCache(k[..., ::2], k[..., ::2]), lambda: nvfp4.PagedBatch(kv.long(), table), lambda: nvfp4.PagedBatch(kv, table[:2]),
+                lambda: nvfp4.PagedBatch(kv, table, cu_q=kv), lambda: nvfp4.PagedBatch(kv.float(), table)]:
+        with pytest.raises(ValueError):
+            bad()

@@ -521,3 +521,19 @@ def test_nothing_to_do(handle):
     handle.kv_append(cache, batch, c.q, c.k, c.v, c.out)
     torch.cuda.synchronize()
     assert bool((c.out == 7).all()) and torch.equal(c.k_cache, k)
+
+
+@pytest.mark.parametrize("dim,q_heads,kv_heads,new", [(256, 24, 2, 2), (256, 12, 4, 9), (256, 6, 1, 5), (128, 32, 8, 8), (128, 6, 2, 7), (128, 17, 1, 1), (64, 16, 4, 6), (64, 20, 1, 1),
+                                                      (64, 32, 1, 1)])
+@pytest.mark.parametrize("page", [16, 24, 5])
+def test_rows_of_two_tiles(handle, dim, q_heads, kv_heads, new, page):
+    """17 to 32 rows a sequence, from one key to parts in many blocks; with and without gates, the second tile full or with a row or two."""
+    past = [0, 3, 31, 32, 33, 63, 64, 127, 500, 3000, 9000]
+    c = ref.Case([new, max(new - 1, 1)] + [new] * (len(past) - 2), past, q_heads, kv_heads, dim, page, seed=dim + new, gate=page == 16, pad=2)
+    check_attention(handle, c, times=2)
+
+
+@pytest.mark.parametrize("dim,q_heads,kv_heads,new", [(256, 24, 2, 2), (128, 32, 8, 8), (64, 20, 1, 1)])
+def test_two_tiles_of_one_long_sequence(handle, dim, q_heads, kv_heads, new):
+    c = ref.Case([new], [40000], q_heads, kv_heads, dim, 32, seed=dim, gate=True)
+    check_attention(handle, c, times=2)
