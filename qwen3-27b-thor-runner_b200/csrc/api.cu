@@ -243,11 +243,11 @@ const char* nvfp4_status_string(int status) {
     switch (status) {
         case NVFP4_OK: return "ok";
         case NVFP4_E_NULL: return "null pointer argument";
-        case NVFP4_E_SHAPE: return "unsupported shape (need M>=0, N>0, K>0, K % 16 == 0)";
-        case NVFP4_E_ALIGN: return "misaligned pointer (A, C, residual: 16 bytes; packed: 8 bytes)";
+        case NVFP4_E_SHAPE: return "unsupported shape (need M>=0, N>0, K>0, K % 16 == 0; paged cache: head_dim 64, 128 or 256, counts and strides as documented)";
+        case NVFP4_E_ALIGN: return "misaligned pointer (A, C, residual: 16 bytes; packed: 8 bytes; paged cache: pointers 16 bytes, strides 8 elements)";
         case NVFP4_E_WORKSPACE: return "handle workspace too small for this call";
-        case NVFP4_E_ALIAS: return "A overlaps the output";
-        case NVFP4_E_SCALE: return "global_scale must be finite and > 0";
+        case NVFP4_E_ALIAS: return "an input overlaps the output";
+        case NVFP4_E_SCALE: return "global_scale must be finite and > 0, the scale of attention finite";
         case NVFP4_E_DEVICE: return "no usable CUDA device (compute capability 10.x required)";
         case NVFP4_E_OPTION: return "unknown option or value";
         case NVFP4_E_TP: return "tensor-parallel set-up error";

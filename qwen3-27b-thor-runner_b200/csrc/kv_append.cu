@@ -4,7 +4,7 @@
 // Every value is read once and written once, and the bound should be that; but a value comes with a dozen instructions, so the instructions
 // are what had to go: with a thread for eight neighbours, partners exchanged by shuffles and addresses formed for every head of every token 6534 tokens of 28
 // heads of 256 took 61-79 us.  Now a head is spread over head_dim / 8 lanes; a lane of the part that turns holds four elements and their partners
-// i + rot_dim / 2, and goes through four tokens with the same head: 46 us, 0.62 of the copy rate.  One token of one sequence takes 2.6 us from a graph, 5.1
+// i + rot_dim / 2, and goes through four tokens with the same head: 46 us, 0.62 of the copy rate.  One token of one sequence takes 2.6 us from a graph, 5.4
 // called, which is the host's.  A norm is a reduction over the head's lanes.  The angles are the same for all heads of a token and computed once, in
 // shared memory, while the loads are under way.
 // position * inv_freq is formed and reduced to [-pi, pi] in FP64 (a float of 2^17 has steps of 1/64: the angle itself would be lost),

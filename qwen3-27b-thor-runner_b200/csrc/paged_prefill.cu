@@ -58,7 +58,7 @@ struct Form {
     static constexpr int kSlots = (224 * 1024 - kNT * kQTile) / kSlotBytes;
     static constexpr int kOCol = 256;                            // scores in front: buffer or tile 0, 1
     static constexpr int kOkRing = 16;                           // units whose page masks are kept: more than the ring holds
-    static constexpr int kControl = 3072;
+    static constexpr int kControl = 3 * 1024;
     static constexpr int kSmem = kNT * kQTile + kSlots * kSlotBytes + kControl;
 };
 static_assert(Form<256>::kSmem <= 232448 && Form<128>::kSmem <= 232448 && Form<64>::kSmem <= 232448, "shared memory");
