@@ -532,7 +532,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
             next_slot();
         }
     } else if (warp <= 2) {
-        // ------------------------------------------------------------------ MMA issuers (leader); the other CTA's two warps wait for the last MMAs
+        // ------------------------------------------------------------------ MMA issuers (leader); the other CTA's two warps go to the end at once
         const bool is_s = warp == 1;
         const uint32_t idesc = 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(2 * kTile >> 4) << 24 | (is_s ? (uint32_t)(kLongChunk >> 3) << 17 : 1u << 16 | (uint32_t)(F::kOCols >> 3) << 17);
         const uint32_t other = ptx::mapa_shared(ptx::smem_u32(full), 1) - ptx::mapa_shared(ptx::smem_u32(full), 0);
@@ -594,7 +594,6 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
             more = at.next_item(p, c0, c1);
         }
         if (rank == 0) commit(&drain[!is_s], other);
-        ptx::mbar_wait(&drain[!is_s], 0, s_abort, b.status, 0xA3Fu);
     } else {
         // ------------------------------------------------------------------ softmax: thread = row and 64 of the scores, half of the result
         const int g = (warp - 3) >> 2, quarter = warp & 3, row = quarter * 32 + lane, s_col = g * 64;
@@ -806,6 +805,10 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
     }
     __syncwarp();
     umma::tc_fence_before();
+    __syncthreads();
+    // The issuers' last MMAs, in both CTAs.  A wait's limit is about a second and a run may take longer, so no wait spans the run: behind the barrier the
+    // softmax warps have read the last item's results, and what is left is the arrival.
+    if (warp == 1 || warp == 2) ptx::mbar_wait(&drain[warp == 2], 0, s_abort, b.status, 0xA3Fu);
     __syncthreads();
     if (*s_abort) {                                  // a wait ran out: nobody issues any more; give what is in flight time to land
         for (int i = 0; i < 200; ++i) __nanosleep(1000);

@@ -53,3 +53,13 @@ def test_what_the_kernel_before_writes_is_not_read_as_read_only():
             if head and "griddep_wait()" not in part:      # an ordinary launch in the same file
                 continue
             assert "__restrict__" not in head and not reads, (name, head, reads)
+
+
+def test_no_wait_of_the_prompt_kernel_spans_a_run():
+    """A wait gives up after about a second; a block's run may take longer.  What a warp waits for at the end, the last MMAs' completion, is waited for behind the
+    barrier that all warps reach with their last item."""
+    src = source("paged_prefill.cu")
+    at = src.index("mbar_wait(&drain[")
+    assert src.count("mbar_wait(&drain[") == 1
+    kernel = src[src.index("paged_prefill_kernel("):at]
+    assert kernel.rfind("__syncthreads();") > kernel.rfind("more = at.next_item(")
