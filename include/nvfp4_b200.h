@@ -344,7 +344,7 @@ typedef struct nvfp4_kv_cache {
  *   max_q_len  the longest run of new tokens to be expected; it selects kernels, a longer run is slower, not wrong.
  * Entries of a table row behind the sequence's last page are not used.  What the device finds out of bounds is left out, and
  * nvfp4_device_status says so (0xA01): a page number outside [0, num_pages) or a position behind table_cols pages takes part in
- * nothing and is not written; cu_q is clamped to [0, tokens].  Sequences may share pages that no new token lies in. */
+ * nothing and is not written; cu_q, which ascends, is clamped to [0, tokens].  Sequences may share pages that no new token lies in. */
 typedef struct nvfp4_paged_batch {
     const int* cu_q;          /* [sequences + 1] or NULL */
     const int* kv_len;        /* [sequences] */

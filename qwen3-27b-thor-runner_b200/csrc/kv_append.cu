@@ -101,6 +101,8 @@ kv_append_kernel(AppendArgs a, int per) {
     };
     begin_head();
     ask(0);
+    // cu_q ascends: its ends tell whether rows outside [0, tokens] are left out
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == kThreads - 1 && b.cu_q && (b.cu_q[0] < 0 || b.cu_q[b.sequences] > b.tokens)) atomicCAS(b.status, 0u, kStatusPlace);
     if (warp < tokens) {
         int seq, pos = 0;
         const bool there = find_row(b, t0 + warp, seq, pos);

@@ -206,6 +206,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         at.q = sequence(b, s);
         at.n = Cursor<D>::items(p, at.q);
         mine += (long long)at.n.items * at.n.cost();
+        // one block says so, the one that is the last to have work of its own
+        if (blockIdx.x + 1 == gridDim.x && cut_off(b, s)) atomicCAS(b.status, 0u, kStatusPlace);
     }
     long long upto = mine;
 #pragma unroll

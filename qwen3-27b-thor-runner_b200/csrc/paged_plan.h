@@ -3,6 +3,7 @@
 #pragma once
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 
 #include "../../include/nvfp4_b200.h"
 
@@ -70,6 +71,16 @@ NVFP4_PAGED_HD Sequence sequence(const Batch& b, int s) {
     r.first = (int)least(most(first, -2147483647LL), 2147483647LL);
     r.kv = least(most(kv, 0), b.max_kv);
     return r;
+}
+
+// Whether sequence() leaves something out: rows outside [0, tokens], or positions behind the table of a sequence that has rows.
+NVFP4_PAGED_HD bool cut_off(const Batch& b, int s) {
+    if (b.cu_q) {
+        const int q0 = b.cu_q[s], q1 = b.cu_q[s + 1];
+        if (q0 < 0 || q1 < q0 || q1 > b.tokens) return true;
+        if (q0 == q1) return false;
+    }
+    return b.kv_len[s] > b.max_kv;
 }
 
 // The keys that new token i of a sequence sees are those in front of this position.

@@ -333,6 +333,8 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
         const Sequence q = sequence(b, s);
         const LongItems n = Cursor<D>::items(p, q);
         mine += long_places(q, n, n.tiles) * n.heads;
+        // one block says so, the one that is the last to have work of its own
+        if (blockIdx.x + 1 == gridDim.x && cut_off(b, s)) atomicCAS(b.status, 0u, kStatusPlace);
     }
     long long upto = mine;
 #pragma unroll

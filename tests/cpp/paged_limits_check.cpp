@@ -1,0 +1,14 @@
+// What the paged cache's calls find out about their arguments (csrc/paged_plan.h), for a test on the CPU.
+#include "paged_plan.h"
+
+using namespace nvfp4::paged;
+
+extern "C" {
+
+// Whether a sequence's rows or positions are cut off; -1: the batch is refused.
+int paged_cut_off(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int s) {
+    Batch x{};
+    return check_batch(c, b, &x) ? -1 : cut_off(x, s);
+}
+
+}  // extern "C"

@@ -38,3 +38,50 @@ def test_a_call_may_take_longer_than_a_wait():
         tol = (steps * 2.0 ** -23 + (row // 128 + 65) * 2.0 ** -24 + ref.BF16_HALF_STEP + score + 2.0 ** -20) * size * (1 + ref.BF16_HALF_STEP) + ref.BF16_HALF_STEP * want.abs()
         assert float(((out[row, 0].double() - want).abs() / tol).max()) <= 1.0, row
     h.close()
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [40, 3, 90], [70, 1, 2, 33]])            # either kernel, and both
+def test_a_length_behind_the_table_is_told(new):
+    """The keys that the table holds take part, and the status says that others did not."""
+    h = nvfp4.Handle(0, 16 << 20)
+    c = ref.Case(new, [200 - n for n in new], 4, 2, 128, 16, seed=len(new), gate=True, pad=2)
+    cache, batch = c.objects(nvfp4)
+    want, tol = ref.attention(c)
+    h.paged_attention(cache, batch, c.q, c.out, gate=c.gate)
+    assert h.device_status() == 0 and ref.worst(c.out, want, tol) <= 1.0
+    # the last sequence: 200 positions of a table of 208, and from the second call on 9 more than it has
+    last = len(new) - 1
+    c.kv_dev[last] = 217
+    h.paged_attention(cache, batch, c.q, c.out, gate=c.gate)
+    assert h.device_status() == 0xA01
+    before = int(c.starts[last])
+    assert ref.worst(c.out[:before], want[:before], tol[:before]) <= 1.0
+    rows = slice(before, before + new[last])
+    k, v = (c.by_token(x)[c.table[last].long().cuda()].flatten(0, 1)[:208].double() for x in (c.k_cache, c.v_cache))
+    for i in range(new[last]):
+        n = min(217 - new[last] + i + 1, 208)
+        for hd in range(4):
+            t = k[:n, hd // 2] @ c.q[before + i, hd].double() * 128 ** -0.5
+            w = torch.softmax(t, 0)
+            o, a = w @ v[:n, hd // 2], w @ v[:n, hd // 2].abs()
+            sig = torch.sigmoid(c.gate[before + i, hd].double())
+            score = 2 * 132 * 2.0 ** -23 * float((k[:n, hd // 2].abs() @ c.q[before + i, hd].double().abs()).max()) * 128 ** -0.5
+            off = (ref.BF16_HALF_STEP + score + 2.0 ** -20) * a * sig * (1 + ref.BF16_HALF_STEP) + ref.BF16_HALF_STEP * (o * sig).abs() + 1e-30
+            assert float(((c.out[before + i, hd].double() - o * sig).abs() / off).max()) <= 1.0
+    assert bool((c.out[rows.stop:] == 7).all())
+    h.close()
+
+
+@pytest.mark.parametrize("starts", [[0, 3, 11], [-1, 3, 8], [0, 50, 90]])
+@pytest.mark.parametrize("call", ["append", "few", "many"])
+def test_rows_outside_the_batch_are_told(starts, call):
+    h = nvfp4.Handle(0, 16 << 20)
+    c = ref.Case([4, 4], [60, 30], 40 if call == "many" else 4, 2, 128, 16, seed=3)
+    cache, batch = c.objects(nvfp4)
+    run = (lambda: h.kv_append(cache, batch, c.q, c.k, c.v, c.out)) if call == "append" else (lambda: h.paged_attention(cache, batch, c.q, c.out))
+    run()
+    assert h.device_status() == 0
+    c.cu_dev.copy_(torch.tensor(starts, dtype=torch.int32))
+    run()
+    assert h.device_status() == 0xA01
+    h.close()
