@@ -175,11 +175,13 @@ class KvCache:
     (order="head") of the same strides, the last one dense."""
 
     def __init__(self, k, v, order="token"):
+        import torch
         token, head = (1, 2) if order == "token" else (2, 1)
         if order not in ("token", "head") or k.shape != v.shape or k.stride() != v.stride() or k.dim() != 4 or k.stride(3) != 1 or \
-                any(t.element_size() != 2 or not t.is_floating_point() for t in (k, v)):
+                any(t.dtype is not torch.bfloat16 for t in (k, v)):
             raise ValueError("k and v: 4-D BF16 tensors of the same shape and strides, the head's values dense; order 'token' or 'head'")
         self.keep = (k, v)
+        self.types = (torch.bfloat16, torch.float32, torch.int32)      # of rows and norms, inv_freq, positions
         self.c = KvCacheStruct(k.data_ptr(), v.data_ptr(), k.shape[0], k.shape[token], k.shape[head], k.shape[3],
                                k.stride(0), k.stride(token), k.stride(head))
         self.address = ctypes.addressof(self.c)
@@ -191,10 +193,11 @@ class PagedBatch:
     are int32 device tensors whose contents may change between calls; tokens (default: one per sequence) and max_q_len are bounds."""
 
     def __init__(self, kv_len, block_table, tokens=None, cu_q=None, max_q_len=1):
+        import torch
         sequences = kv_len.shape[0]
-        for t in (kv_len, block_table, cu_q):
-            if t is not None and (t.element_size() != 4 or t.is_floating_point() or t.stride(-1) != 1):
-                raise ValueError("kv_len, block_table and cu_q are dense int32 tensors")
+        for t, dim in ((kv_len, 1), (block_table, 2), (cu_q, 1)):
+            if t is not None and (t.dtype is not torch.int32 or t.dim() != dim or t.stride(-1) != 1):
+                raise ValueError("kv_len [sequences], block_table [sequences, columns] and cu_q [sequences + 1] are dense int32 tensors")
         if block_table.shape[0] != sequences or (cu_q is not None and cu_q.shape[0] != sequences + 1):
             raise ValueError("block_table has a row per sequence, cu_q an entry more than there are sequences")
         self.keep = (kv_len, block_table, cu_q)
@@ -211,13 +214,16 @@ assert _APPEND.size == ctypes.sizeof(KvAppendDesc) and _ATTENTION.size == ctypes
 _NO_ROWS = (0, 0, 0, 0)
 
 
-def _rows(t, tokens, dim):
+def _rows(t, tokens, dim, dtype):
     """Address, token stride, head stride and heads of a [tokens, heads, head dim] tensor."""
     n, heads, d = t.shape
     a, b, c = t.stride()
-    if c != 1 or a == 0 or b == 0 or n < tokens or d != dim:       # a stride of 0 would mean dense
-        raise ValueError("a [tokens, heads, head dim] tensor with the batch's tokens and the cache's head dim, whose heads are dense and that repeats nothing")
+    if c != 1 or a == 0 or b == 0 or n < tokens or d != dim or t.dtype is not dtype:       # a stride of 0 would mean dense
+        raise ValueError("a BF16 tensor [tokens, heads, head dim] with the batch's tokens and the cache's head dim, whose heads are dense and that repeats nothing")
     return t.data_ptr(), a, b, heads
+
+
+_VECTORS = "norms are dense BF16 tensors of a head's values, inv_freq a dense FP32 one, positions a dense int32 one with a value a token"
 
 
 class Handle:
@@ -338,23 +344,42 @@ class Handle:
         """nvfp4_kv_append: norms, rotation (of 2 * len(inv_freq) elements) and append.  q, k, v and q_out are [tokens, heads, head dim] tensors
         (views with strides are fine; q and q_out None: keys and values only)."""
         tokens, dim = batch.tokens, cache.dim
-        qp, qt, qh, heads = _NO_ROWS if q is None else _rows(q, tokens, dim)
-        op, ot, oh, out_heads = _NO_ROWS if q is None else _rows(q_out, tokens, dim)
-        kp, kt, kh, k_heads = _rows(k, tokens, dim)
-        vp, vt, vh, v_heads = _rows(v, tokens, dim)
+        bf16, fp32, int32 = cache.types
+        if q is not None and q_out is None:
+            raise ValueError("q needs a q_out")
+        qp, qt, qh, heads = _NO_ROWS if q is None else _rows(q, tokens, dim, bf16)
+        op, ot, oh, out_heads = _NO_ROWS if q is None else _rows(q_out, tokens, dim, bf16)
+        kp, kt, kh, k_heads = _rows(k, tokens, dim, bf16)
+        vp, vt, vh, v_heads = _rows(v, tokens, dim, bf16)
         if heads != out_heads or k_heads != cache.heads or v_heads != cache.heads:
             raise ValueError("q and q_out have the same heads, k and v the cache's")
-        d = _APPEND.pack(cache.address, batch.address, qp, kp, vp, op, qt, qh, kt, kh, vt, vh, ot, oh, 0 if q_norm is None else q_norm.data_ptr(),
-                         0 if k_norm is None else k_norm.data_ptr(), 0 if inv_freq is None else inv_freq.data_ptr(), 0 if positions is None else positions.data_ptr(),
-                         heads, 0 if inv_freq is None else 2 * inv_freq.numel(), norm_eps)
+        qn = kn = freq = pos = rot_dim = 0
+        if q_norm is not None:
+            if q_norm.dtype is not bf16 or q_norm.numel() != dim or not q_norm.is_contiguous():
+                raise ValueError(_VECTORS)
+            qn = q_norm.data_ptr()
+        if k_norm is not None:
+            if k_norm.dtype is not bf16 or k_norm.numel() != dim or not k_norm.is_contiguous():
+                raise ValueError(_VECTORS)
+            kn = k_norm.data_ptr()
+        if inv_freq is not None:
+            if inv_freq.dtype is not fp32 or not inv_freq.is_contiguous():
+                raise ValueError(_VECTORS)
+            freq, rot_dim = inv_freq.data_ptr(), 2 * inv_freq.numel()
+        if positions is not None:
+            if positions.dtype is not int32 or positions.numel() < tokens or not positions.is_contiguous():
+                raise ValueError(_VECTORS)
+            pos = positions.data_ptr()
+        d = _APPEND.pack(cache.address, batch.address, qp, kp, vp, op, qt, qh, kt, kh, vt, vh, ot, oh, qn, kn, freq, pos, heads, rot_dim, norm_eps)
         self._check(self.lib.nvfp4_kv_append(self.h, d, _stream(stream)))
 
     def paged_attention(self, cache, batch, q, out, gate=None, scale=0.0, stream=None):
         """nvfp4_paged_attention: q, out and gate are [tokens, heads, head dim] tensors; scale 0 = 1 / sqrt(head dim)."""
         tokens, dim = batch.tokens, cache.dim
-        qp, qt, qh, heads = _rows(q, tokens, dim)
-        op, ot, oh, out_heads = _rows(out, tokens, dim)
-        gp, gt, gh, gate_heads = (0, 0, 0, heads) if gate is None else _rows(gate, tokens, dim)
+        bf16 = cache.types[0]
+        qp, qt, qh, heads = _rows(q, tokens, dim, bf16)
+        op, ot, oh, out_heads = _rows(out, tokens, dim, bf16)
+        gp, gt, gh, gate_heads = (0, 0, 0, heads) if gate is None else _rows(gate, tokens, dim, bf16)
         if not heads == out_heads == gate_heads:
             raise ValueError("q, out and gate have the same heads")
         d = _ATTENTION.pack(cache.address, batch.address, qp, gp, op, qt, qh, gt, gh, ot, oh, heads, scale)

@@ -5,7 +5,9 @@ import random
 import subprocess
 
 import pytest
+import torch
 
+import nvfp4
 import test_paged_cpu as base
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -38,3 +40,76 @@ def test_what_is_cut_off_is_noticed(lib):
     assert min(seen) > 200
     c, b = base.arrays([32, 33, 0, -1], [[0, 1]] * 4, page_size=16)            # a token a sequence
     assert [lib.paged_cut_off(ctypes.byref(c), ctypes.byref(b), s) for s in range(4)] == [0, 1, 0, 0]
+
+
+class _Library:
+    """Stands in for the library: keeps the descriptors that reach it."""
+
+    def __init__(self):
+        self.got = []
+
+    def nvfp4_kv_append(self, handle, d, stream):
+        self.got.append(nvfp4.KvAppendDesc.from_buffer_copy(d))
+        return 0
+
+    def nvfp4_paged_attention(self, handle, d, stream):
+        self.got.append(nvfp4.PagedAttentionDesc.from_buffer_copy(d))
+        return 0
+
+
+def _bound(tokens=3, dim=64):
+    """A handle on the stand-in, a cache and a batch of CPU tensors, and a function that makes zeros."""
+    h = object.__new__(nvfp4.Handle)
+    h.h, h.lib = None, _Library()
+    new = lambda *s, dtype=torch.bfloat16: torch.zeros(s, dtype=dtype)
+    k = new(4, 16, 2, dim)
+    batch = nvfp4.PagedBatch(torch.ones(tokens, dtype=torch.int32), torch.zeros(tokens, 2, dtype=torch.int32))
+    return h, nvfp4.KvCache(k, k.clone()), batch, new
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.int16, torch.float64])
+def test_the_binding_refuses_other_types_of_rows(dtype):
+    h, cache, batch, new = _bound()
+    with pytest.raises(ValueError):
+        nvfp4.KvCache(new(4, 16, 2, 64, dtype=dtype), new(4, 16, 2, 64, dtype=dtype))
+    rows = [new(3, 6, 64), new(3, 2, 64), new(3, 2, 64), new(3, 6, 64)]
+    for i in range(4):
+        bad = list(rows)
+        bad[i] = bad[i].to(dtype)
+        with pytest.raises(ValueError):
+            h.kv_append(cache, batch, *bad, stream=0)
+    q, out, gate = rows[0], rows[3], new(3, 6, 64)
+    for args, kw in [((q.to(dtype), out), {}), ((q, out.to(dtype)), {}), ((q, out), {"gate": gate.to(dtype)})]:
+        with pytest.raises(ValueError):
+            h.paged_attention(cache, batch, *args, stream=0, **kw)
+    assert not h.lib.got
+
+
+def test_the_binding_refuses_vectors_that_do_not_fit():
+    """Norms, frequencies and positions are read by the device without a look at what they are."""
+    h, cache, batch, new = _bound()
+    q, k, v, out = new(3, 6, 64), new(3, 2, 64), new(3, 2, 64), new(3, 6, 64)
+    good = {"q_norm": new(64), "k_norm": new(64), "inv_freq": torch.ones(16), "positions": torch.arange(3, dtype=torch.int32)}
+    h.kv_append(cache, batch, q, k, v, out, stream=0, **good)
+    h.kv_append(cache, batch, q, k, v, out, stream=0)
+    h.kv_append(cache, batch, None, k, v, None, stream=0, positions=torch.arange(9, dtype=torch.int32))
+    assert [(d.q_norm, d.k_norm, d.inv_freq, d.positions) for d in h.lib.got[:2]] == [tuple(t.data_ptr() for t in good.values()), (None,) * 4]
+    assert [(d.q_heads, d.rot_dim) for d in h.lib.got] == [(6, 32), (6, 0), (0, 0)]
+    reached = len(h.lib.got)
+    for name in ("q_norm", "k_norm"):
+        for bad in [new(64, dtype=torch.float32), new(64, dtype=torch.float16), new(63), new(128), new(128)[::2], new(0)]:
+            with pytest.raises(ValueError):
+                h.kv_append(cache, batch, q, k, v, out, stream=0, **{**good, name: bad})
+    for bad in [torch.ones(16, dtype=torch.float64), torch.ones(32)[::2], new(16)]:
+        with pytest.raises(ValueError):
+            h.kv_append(cache, batch, q, k, v, out, stream=0, **{**good, "inv_freq": bad})
+    for bad in [torch.arange(3), torch.arange(2, dtype=torch.int32), torch.arange(6, dtype=torch.int32)[::2], torch.ones(3), torch.arange(3, dtype=torch.int16)]:
+        with pytest.raises(ValueError):
+            h.kv_append(cache, batch, q, k, v, out, stream=0, **{**good, "positions": bad})
+    with pytest.raises(ValueError):
+        h.kv_append(cache, batch, q, k, v, None, stream=0)
+    kv, table = torch.ones(3, dtype=torch.int32), torch.zeros(3, 2, dtype=torch.int32)
+    for args in [(kv.view(3, 1), table), (kv, torch.zeros(3, dtype=torch.int32)), (kv.to(torch.uint32), table), (kv, table.to(torch.uint32))]:
+        with pytest.raises((ValueError, IndexError)):
+            nvfp4.PagedBatch(*args)
+    assert len(h.lib.got) == reached
