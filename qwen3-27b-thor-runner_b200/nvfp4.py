@@ -190,7 +190,8 @@ class KvCache:
 
 class PagedBatch:
     """nvfp4_paged_batch: kv_len [sequences], block_table [sequences, columns] and cu_q [sequences + 1] (None: one new token per sequence)
-    are int32 device tensors whose contents may change between calls; tokens (default: one per sequence) and max_q_len are bounds."""
+    are int32 device tensors whose contents may change between calls; tokens (with cu_q the rows of q, k, v and out; without it one per
+    sequence unless it says more) and max_q_len are bounds."""
 
     def __init__(self, kv_len, block_table, tokens=None, cu_q=None, max_q_len=1):
         import torch
@@ -200,6 +201,8 @@ class PagedBatch:
                 raise ValueError("kv_len [sequences], block_table [sequences, columns] and cu_q [sequences + 1] are dense int32 tensors")
         if block_table.shape[0] != sequences or (cu_q is not None and cu_q.shape[0] != sequences + 1):
             raise ValueError("block_table has a row per sequence, cu_q an entry more than there are sequences")
+        if cu_q is not None and tokens is None:             # rows behind `tokens` take part in nothing, and how many there are is on the device
+            raise ValueError("cu_q comes with tokens")
         self.keep = (kv_len, block_table, cu_q)
         self.c = PagedBatchStruct(_ptr(cu_q), kv_len.data_ptr(), block_table.data_ptr(), block_table.stride(0), block_table.shape[1], sequences,
                                   sequences if tokens is None else tokens, max_q_len)

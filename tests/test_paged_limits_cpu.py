@@ -113,3 +113,12 @@ def test_the_binding_refuses_vectors_that_do_not_fit():
         with pytest.raises((ValueError, IndexError)):
             nvfp4.PagedBatch(*args)
     assert len(h.lib.got) == reached
+
+
+def test_offsets_come_with_the_number_of_rows():
+    """One row per sequence, the default without offsets, would leave out most of a prompt without a word."""
+    kv, table, cu = torch.full((3,), 40, dtype=torch.int32), torch.zeros(3, 4, dtype=torch.int32), torch.tensor([0, 20, 21, 30], dtype=torch.int32)
+    with pytest.raises(ValueError):
+        nvfp4.PagedBatch(kv, table, cu_q=cu, max_q_len=20)
+    assert nvfp4.PagedBatch(kv, table, tokens=30, cu_q=cu, max_q_len=20).tokens == 30
+    assert nvfp4.PagedBatch(kv, table).tokens == 3 and nvfp4.PagedBatch(kv, table, tokens=5).tokens == 5
