@@ -177,11 +177,12 @@ class KvCache:
     def __init__(self, k, v, order="token"):
         import torch
         token, head = (1, 2) if order == "token" else (2, 1)
-        if order not in ("token", "head") or k.shape != v.shape or k.stride() != v.stride() or k.dim() != 4 or k.stride(3) != 1 or \
+        if order not in ("token", "head") or k.get_device() != v.get_device() or k.shape != v.shape or k.stride() != v.stride() or k.dim() != 4 or k.stride(3) != 1 or \
                 any(t.dtype is not torch.bfloat16 for t in (k, v)):
-            raise ValueError("k and v: 4-D BF16 tensors of the same shape and strides, the head's values dense; order 'token' or 'head'")
+            raise ValueError("k and v: 4-D BF16 tensors of a device and of the same shape and strides, the head's values dense; order 'token' or 'head'")
         self.keep = (k, v)
         self.types = (torch.bfloat16, torch.float32, torch.int32)      # of rows and norms, inv_freq, positions
+        self.device = k.get_device()
         self.c = KvCacheStruct(k.data_ptr(), v.data_ptr(), k.shape[0], k.shape[token], k.shape[head], k.shape[3],
                                k.stride(0), k.stride(token), k.stride(head))
         self.address = ctypes.addressof(self.c)
@@ -197,8 +198,8 @@ class PagedBatch:
         import torch
         sequences = kv_len.shape[0]
         for t, dim in ((kv_len, 1), (block_table, 2), (cu_q, 1)):
-            if t is not None and (t.dtype is not torch.int32 or t.dim() != dim or t.stride(-1) != 1):
-                raise ValueError("kv_len [sequences], block_table [sequences, columns] and cu_q [sequences + 1] are dense int32 tensors")
+            if t is not None and (t.dtype is not torch.int32 or t.dim() != dim or t.stride(-1) != 1 or t.get_device() != kv_len.get_device()):
+                raise ValueError("kv_len [sequences], block_table [sequences, columns] and cu_q [sequences + 1] are dense int32 tensors of a device")
         if block_table.shape[0] != sequences or (cu_q is not None and cu_q.shape[0] != sequences + 1):
             raise ValueError("block_table has a row per sequence, cu_q an entry more than there are sequences")
         if cu_q is not None and tokens is None:             # rows behind `tokens` take part in nothing, and how many there are is on the device
@@ -208,6 +209,7 @@ class PagedBatch:
                                   sequences if tokens is None else tokens, max_q_len)
         self.address = ctypes.addressof(self.c)
         self.tokens = self.c.tokens
+        self.device = kv_len.get_device()
 
 
 # The descriptors of the calls on a paged cache as bytes: packing them takes a third of the time that filling a ctypes structure does.
@@ -217,16 +219,17 @@ assert _APPEND.size == ctypes.sizeof(KvAppendDesc) and _ATTENTION.size == ctypes
 _NO_ROWS = (0, 0, 0, 0)
 
 
-def _rows(t, tokens, dim, dtype):
+def _rows(t, tokens, dim, dtype, device):
     """Address, token stride, head stride and heads of a [tokens, heads, head dim] tensor."""
     n, heads, d = t.shape
     a, b, c = t.stride()
-    if c != 1 or a == 0 or b == 0 or n < tokens or d != dim or t.dtype is not dtype:       # a stride of 0 would mean dense
-        raise ValueError("a BF16 tensor [tokens, heads, head dim] with the batch's tokens and the cache's head dim, whose heads are dense and that repeats nothing")
+    if c != 1 or a == 0 or b == 0 or n < tokens or d != dim or t.dtype is not dtype or t.get_device() != device:       # a stride of 0 would mean dense
+        raise ValueError("a BF16 tensor [tokens, heads, head dim] on the cache's device with the batch's tokens and the cache's head dim, whose heads are dense and that "
+                         "repeats nothing")
     return t.data_ptr(), a, b, heads
 
 
-_VECTORS = "norms are dense BF16 tensors of a head's values, inv_freq a dense FP32 one, positions a dense int32 one with a value a token"
+_VECTORS = "norms are dense BF16 tensors of a head's values, inv_freq a dense FP32 one, positions a dense int32 one with a value a token, on the cache's device"
 
 
 class Handle:
@@ -239,6 +242,7 @@ class Handle:
         if st:
             raise Nvfp4Error(st)
         self.h = h
+        self.device = device
 
     def close(self):
         if getattr(self, "h", None):
@@ -346,31 +350,33 @@ class Handle:
     def kv_append(self, cache, batch, q, k, v, q_out, q_norm=None, k_norm=None, norm_eps=1e-6, inv_freq=None, positions=None, stream=None):
         """nvfp4_kv_append: norms, rotation (of 2 * len(inv_freq) elements) and append.  q, k, v and q_out are [tokens, heads, head dim] tensors
         (views with strides are fine; q and q_out None: keys and values only)."""
-        tokens, dim = batch.tokens, cache.dim
+        tokens, dim, device = batch.tokens, cache.dim, cache.device
         bf16, fp32, int32 = cache.types
         if q is not None and q_out is None:
             raise ValueError("q needs a q_out")
-        qp, qt, qh, heads = _NO_ROWS if q is None else _rows(q, tokens, dim, bf16)
-        op, ot, oh, out_heads = _NO_ROWS if q is None else _rows(q_out, tokens, dim, bf16)
-        kp, kt, kh, k_heads = _rows(k, tokens, dim, bf16)
-        vp, vt, vh, v_heads = _rows(v, tokens, dim, bf16)
+        qp, qt, qh, heads = _NO_ROWS if q is None else _rows(q, tokens, dim, bf16, device)
+        op, ot, oh, out_heads = _NO_ROWS if q is None else _rows(q_out, tokens, dim, bf16, device)
+        kp, kt, kh, k_heads = _rows(k, tokens, dim, bf16, device)
+        vp, vt, vh, v_heads = _rows(v, tokens, dim, bf16, device)
         if heads != out_heads or k_heads != cache.heads or v_heads != cache.heads:
             raise ValueError("q and q_out have the same heads, k and v the cache's")
+        if device != self.device or batch.device != device:
+            raise ValueError("cache and batch are on the handle's device")
         qn = kn = freq = pos = rot_dim = 0
         if q_norm is not None:
-            if q_norm.dtype is not bf16 or q_norm.numel() != dim or not q_norm.is_contiguous():
+            if q_norm.dtype is not bf16 or q_norm.numel() != dim or not q_norm.is_contiguous() or q_norm.get_device() != device:
                 raise ValueError(_VECTORS)
             qn = q_norm.data_ptr()
         if k_norm is not None:
-            if k_norm.dtype is not bf16 or k_norm.numel() != dim or not k_norm.is_contiguous():
+            if k_norm.dtype is not bf16 or k_norm.numel() != dim or not k_norm.is_contiguous() or k_norm.get_device() != device:
                 raise ValueError(_VECTORS)
             kn = k_norm.data_ptr()
         if inv_freq is not None:
-            if inv_freq.dtype is not fp32 or not inv_freq.is_contiguous():
+            if inv_freq.dtype is not fp32 or not inv_freq.is_contiguous() or inv_freq.get_device() != device:
                 raise ValueError(_VECTORS)
             freq, rot_dim = inv_freq.data_ptr(), 2 * inv_freq.numel()
         if positions is not None:
-            if positions.dtype is not int32 or positions.numel() < tokens or not positions.is_contiguous():
+            if positions.dtype is not int32 or positions.numel() < tokens or not positions.is_contiguous() or positions.get_device() != device:
                 raise ValueError(_VECTORS)
             pos = positions.data_ptr()
         d = _APPEND.pack(cache.address, batch.address, qp, kp, vp, op, qt, qh, kt, kh, vt, vh, ot, oh, qn, kn, freq, pos, heads, rot_dim, norm_eps)
@@ -378,13 +384,15 @@ class Handle:
 
     def paged_attention(self, cache, batch, q, out, gate=None, scale=0.0, stream=None):
         """nvfp4_paged_attention: q, out and gate are [tokens, heads, head dim] tensors; scale 0 = 1 / sqrt(head dim)."""
-        tokens, dim = batch.tokens, cache.dim
+        tokens, dim, device = batch.tokens, cache.dim, cache.device
         bf16 = cache.types[0]
-        qp, qt, qh, heads = _rows(q, tokens, dim, bf16)
-        op, ot, oh, out_heads = _rows(out, tokens, dim, bf16)
-        gp, gt, gh, gate_heads = (0, 0, 0, heads) if gate is None else _rows(gate, tokens, dim, bf16)
+        qp, qt, qh, heads = _rows(q, tokens, dim, bf16, device)
+        op, ot, oh, out_heads = _rows(out, tokens, dim, bf16, device)
+        gp, gt, gh, gate_heads = (0, 0, 0, heads) if gate is None else _rows(gate, tokens, dim, bf16, device)
         if not heads == out_heads == gate_heads:
             raise ValueError("q, out and gate have the same heads")
+        if device != self.device or batch.device != device:
+            raise ValueError("cache and batch are on the handle's device")
         d = _ATTENTION.pack(cache.address, batch.address, qp, gp, op, qt, qh, gt, gh, ot, oh, heads, scale)
         self._check(self.lib.nvfp4_paged_attention(self.h, d, _stream(stream)))
 

@@ -60,7 +60,7 @@ class _Library:
 def _bound(tokens=3, dim=64):
     """A handle on the stand-in, a cache and a batch of CPU tensors, and a function that makes zeros."""
     h = object.__new__(nvfp4.Handle)
-    h.h, h.lib = None, _Library()
+    h.h, h.lib, h.device = None, _Library(), -1          # the device that CPU tensors name
     new = lambda *s, dtype=torch.bfloat16: torch.zeros(s, dtype=dtype)
     k = new(4, 16, 2, dim)
     batch = nvfp4.PagedBatch(torch.ones(tokens, dtype=torch.int32), torch.zeros(tokens, 2, dtype=torch.int32))
@@ -122,3 +122,37 @@ def test_offsets_come_with_the_number_of_rows():
         nvfp4.PagedBatch(kv, table, cu_q=cu, max_q_len=20)
     assert nvfp4.PagedBatch(kv, table, tokens=30, cu_q=cu, max_q_len=20).tokens == 30
     assert nvfp4.PagedBatch(kv, table).tokens == 3 and nvfp4.PagedBatch(kv, table, tokens=5).tokens == 5
+
+
+def test_the_binding_refuses_tensors_of_other_devices():
+    """An address of the host's memory, or of another device's, would be read by the handle's device."""
+    h, cache, batch, new = _bound()
+    rows = [new(3, 6, 64), new(3, 2, 64), new(3, 2, 64), new(3, 6, 64)]
+    h.kv_append(cache, batch, *rows, stream=0)
+    h.paged_attention(cache, batch, rows[0], rows[3], stream=0)
+    assert len(h.lib.got) == 2
+    for on in [(0, -1, -1), (-1, 0, -1), (-1, -1, 0), (0, 0, -1), (0, 0, 0)]:           # of the handle, the cache and the batch; rows stay on the CPU
+        h.device, cache.device, batch.device = on
+        with pytest.raises(ValueError):
+            h.kv_append(cache, batch, *rows, stream=0)
+        with pytest.raises(ValueError):
+            h.paged_attention(cache, batch, rows[0], rows[3], stream=0)
+    assert len(h.lib.got) == 2
+    h.device = cache.device = batch.device = -1
+    for vector in ({"q_norm": new(64)}, {"inv_freq": torch.ones(16)}, {"positions": torch.arange(3, dtype=torch.int32)}):
+        h.kv_append(cache, batch, *rows, stream=0, **vector)
+        with pytest.raises(ValueError):
+            h.kv_append(cache, batch, *rows, stream=0, **{n: _Elsewhere(t) for n, t in vector.items()})
+
+
+class _Elsewhere:
+    """A tensor that says it is on device 3."""
+
+    def __init__(self, t):
+        self.t = t
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+    def get_device(self):
+        return 3
