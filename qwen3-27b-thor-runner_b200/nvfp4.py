@@ -155,7 +155,8 @@ def _ptr(t):
 _raw_stream = None
 
 
-def _stream(stream):
+def _stream(stream, device=None):
+    """Address of a stream; None: the current one of a device, by default of the current device."""
     if stream is None:
         global _raw_stream
         if _raw_stream is None:
@@ -163,8 +164,8 @@ def _stream(stream):
             torch.cuda.init()
             # the address alone, where torch gives it: building a Stream object takes 3 us of a call's 9
             get, dev = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
-            _raw_stream = (lambda: get(dev())) if get and dev else (lambda: torch.cuda.current_stream().cuda_stream)
-        return _raw_stream()
+            _raw_stream = (lambda d: get(dev() if d is None else d)) if get and dev else (lambda d: torch.cuda.current_stream(d).cuda_stream)
+        return _raw_stream(device)
     if isinstance(stream, int):
         return stream
     return stream.cuda_stream
@@ -380,7 +381,7 @@ class Handle:
                 raise ValueError(_VECTORS)
             pos = positions.data_ptr()
         d = _APPEND.pack(cache.address, batch.address, qp, kp, vp, op, qt, qh, kt, kh, vt, vh, ot, oh, qn, kn, freq, pos, heads, rot_dim, norm_eps)
-        self._check(self.lib.nvfp4_kv_append(self.h, d, _stream(stream)))
+        self._check(self.lib.nvfp4_kv_append(self.h, d, _stream(stream, device)))
 
     def paged_attention(self, cache, batch, q, out, gate=None, scale=0.0, stream=None):
         """nvfp4_paged_attention: q, out and gate are [tokens, heads, head dim] tensors; scale 0 = 1 / sqrt(head dim)."""
@@ -394,7 +395,7 @@ class Handle:
         if device != self.device or batch.device != device:
             raise ValueError("cache and batch are on the handle's device")
         d = _ATTENTION.pack(cache.address, batch.address, qp, gp, op, qt, qh, gt, gh, ot, oh, heads, scale)
-        self._check(self.lib.nvfp4_paged_attention(self.h, d, _stream(stream)))
+        self._check(self.lib.nvfp4_paged_attention(self.h, d, _stream(stream, device)))
 
     def linear_host(self, A_host, M, packed, scale, global_scale, N, K, C_host, residual_host=None, stream=None):
         self._check(self.lib.nvfp4_linear_host(self.h, _ptr(A_host), M, _ptr(packed), _ptr(scale), global_scale,

@@ -156,3 +156,15 @@ class _Elsewhere:
 
     def get_device(self):
         return 3
+
+
+def test_the_current_stream_is_that_of_the_handles_device(monkeypatch):
+    """The calls run on the handle's device, whichever is current; so does the stream that they take where none is given."""
+    h, cache, batch, new = _bound()
+    asked = []
+    monkeypatch.setattr(nvfp4, "_raw_stream", lambda *device: asked.append(device) or 7)
+    rows = [new(3, 6, 64), new(3, 2, 64), new(3, 2, 64), new(3, 6, 64)]
+    h.kv_append(cache, batch, *rows)
+    h.paged_attention(cache, batch, rows[0], rows[3])
+    assert asked == [(-1,), (-1,)]
+    assert nvfp4._stream(None) == 7 and asked[2] == (None,) and nvfp4._stream(5) == 5
