@@ -210,6 +210,46 @@ inline Span span_of(const void* p, long long rows, long long stride, long long h
     const uintptr_t c = reinterpret_cast<uintptr_t>(p);
     return {c, c + (uintptr_t)((rows - 1) * stride + (heads - 1) * head_stride + dim) * 2};
 }
+// Indices lo .. hi of a stride.
+struct Steps {
+    long long stride, lo, hi;
+};
+inline long long floor_quotient(long long a, long long b) { return a / b - (a % b != 0 && a < 0); }
+// Whether two runs of `dim` values whose distance is d and some index of each of n strides (above 0) have a value in common.  Exact: of the largest
+// stride only the indices are tried that the others can still bring near, which is one or two where the strides are nested, as those of rows are.  A search
+// of more than `budget` steps, which takes strides that no layout has, counts as found.
+inline bool meet(long long d, const Steps* t, int n, int dim, int& budget) {
+    if (--budget < 0) return true;
+    if (n == 0) return d > -dim && d < dim;
+    long long low = 0, high = 0;
+    for (int i = 1; i < n; ++i) {
+        low += t[i].stride * t[i].lo;
+        high += t[i].stride * t[i].hi;
+    }
+    // -dim < d + i * stride + (low .. high) < dim
+    const long long from = most(floor_quotient(-dim - d - high, t->stride) + 1, t->lo), to = least(-floor_quotient(d + low - dim, t->stride) - 1, t->hi);
+    for (long long i = from; i <= to; ++i)
+        if (meet(d + i * t->stride, t + 1, n - 1, dim, budget)) return true;
+    return false;
+}
+inline bool meet(long long d, std::initializer_list<Steps> strides, int dim) {
+    Steps t[4];
+    int n = 0, budget = 1 << 16;
+    for (const Steps& x : strides) {
+        if (x.lo == 0 && x.hi == 0) continue;
+        int i = n++;
+        for (; i > 0 && t[i - 1].stride < x.stride; --i) t[i] = t[i - 1];
+        t[i] = x;
+    }
+    return meet(d, t, n, dim, budget);
+}
+// Two tensors of `rows` rows whose spans overlap: whether they share a value.
+inline bool rows_meet(const void* p, long long stride, long long heads, long long head_stride, const void* q, long long q_stride, long long q_heads, long long q_head_stride,
+                      long long rows, int dim) {
+    const long long d = (static_cast<const char*>(p) - static_cast<const char*>(q)) / 2;
+    if (stride == q_stride) return meet(d, {{stride, 1 - rows, rows - 1}, {head_stride, 0, heads - 1}, {q_head_stride, 1 - q_heads, 0}}, dim);
+    return meet(d, {{stride, 0, rows - 1}, {q_stride, 1 - rows, 0}, {head_stride, 0, heads - 1}, {q_head_stride, 1 - q_heads, 0}}, dim);
+}
 // n steps of a stride stay far from the end of 64 bits
 inline bool fits(long long n, long long stride) { return n <= 0 || stride <= (1LL << 46) / n; }
 
@@ -303,6 +343,9 @@ inline int check_append(const nvfp4_kv_append_desc* d, AppendArgs* out, bool* em
     const Span k = span_of(a.k, tokens, a.k_stride, a.b.kv_heads, a.k_head, dim), v = span_of(a.v, tokens, a.v_stride, a.b.kv_heads, a.v_head, dim);
     const Span ck = span_of_cache(a.b, a.b.k), cv = span_of_cache(a.b, a.b.v);
     if (!in_place && (o.overlaps(q) || o.overlaps(k) || o.overlaps(v))) return NVFP4_E_ALIAS;
+    // in place keys and values may lie between q's rows and heads, as a merged projection leaves them, but not in them
+    if (in_place && o.overlaps(k) && rows_meet(a.q_out, a.o_stride, d->q_heads, a.o_head, a.k, a.k_stride, a.b.kv_heads, a.k_head, tokens, dim)) return NVFP4_E_ALIAS;
+    if (in_place && o.overlaps(v) && rows_meet(a.q_out, a.o_stride, d->q_heads, a.o_head, a.v, a.v_stride, a.b.kv_heads, a.v_head, tokens, dim)) return NVFP4_E_ALIAS;
     for (const Span& x : {q, k, v, o})
         if (x.overlaps(ck) || x.overlaps(cv)) return NVFP4_E_ALIAS;
     a.q_norm = static_cast<const uint16_t*>(d->q_norm);

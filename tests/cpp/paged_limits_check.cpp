@@ -11,4 +11,15 @@ int paged_cut_off(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int s) {
     return check_batch(c, b, &x) ? -1 : cut_off(x, s);
 }
 
+int limits_check_append(const nvfp4_kv_append_desc* d) {
+    AppendArgs a{};
+    bool empty = false;
+    return check_append(d, &a, &empty);
+}
+int limits_check_attention(const nvfp4_paged_attention_desc* d) {
+    AttentionArgs a{};
+    bool empty = false;
+    return check_attention(d, &a, &empty);
+}
+
 }  // extern "C"

@@ -168,3 +168,42 @@ def test_the_current_stream_is_that_of_the_handles_device(monkeypatch):
     h.paged_attention(cache, batch, rows[0], rows[3])
     assert asked == [(-1,), (-1,)]
     assert nvfp4._stream(None) == 7 and asked[2] == (None,) and nvfp4._stream(5) == 5
+
+
+def _values(at, rows, stride, heads, head_stride, dim):
+    """The value numbers of a [rows][heads][dim] tensor."""
+    return [at + r * stride + h * head_stride + i for r in range(rows) for h in range(heads) for i in range(dim)]
+
+
+def test_keys_and_values_in_the_rows_of_queries_in_place(lib):
+    """In place, keys and values may lie between q's rows and heads but not in them: against the sets of all values' places."""
+    rng = random.Random(8)
+    at, found = 1 << 22, [0, 0]
+    for _ in range(1500):
+        dim, rows, heads, kv_heads = 64, rng.choice([1, 2, 3, 5, 9]), rng.choice([1, 2, 3, 6]), rng.choice([1, 2, 3])
+        heads = heads * kv_heads
+        head = rng.choice([64, 64, 128, 136, 192])
+        stride = rng.choice([(heads - 1) * head + 64, heads * head + kv_heads * 128, heads * head + 8 * rng.randint(0, 200)])
+        k_head = rng.choice([64, 64, 72, 128, head, head])
+        k_stride = rng.choice([stride, stride, stride, stride + 8, 2 * stride, 64 * kv_heads, k_head * kv_heads])
+        k_at = 8 * rng.randint(-40, (rows * stride + heads * head) // 8 + 40)
+        c = base.cache(k=1 << 30, v=1 << 31, head_dim=dim, kv_heads=kv_heads, head_stride=64, token_stride=64 * kv_heads, page_stride=16 * 64 * kv_heads)
+        b = base.batch(tokens=rows)
+        q = _values(0, rows, stride, heads, head, dim)
+        want = not set(q).isdisjoint(_values(k_at, rows, k_stride, kv_heads, k_head, dim))
+        for name, other in (("k", "v"), ("v", "k")):
+            d = base.append_desc(c, b, q=at, q_out=at, q_heads=heads, rot_dim=0, q_stride=stride, q_head_stride=head, q_out_stride=stride, q_out_head_stride=head,
+                                 **{name: at + 2 * k_at, name + "_stride": k_stride, name + "_head_stride": k_head, other: 1 << 26, other + "_stride": 64 * kv_heads})
+            assert lib.limits_check_append(ctypes.byref(d)) == (base.E_ALIAS if want else 0), (rows, heads, head, stride, kv_heads, k_head, k_stride, k_at)
+        found[want] += 1
+    assert min(found) > 200
+    # as a merged projection leaves them, 8192 tokens: q and gate head by head, then keys, then values
+    c, b = base.cache(head_dim=256, head_stride=256, token_stride=512, page_stride=8192, k=1 << 40, v=1 << 41), base.batch(tokens=8192)
+    row = (48 + 4) * 256
+    good = dict(q=at, q_out=at, q_heads=24, rot_dim=0, q_stride=row, q_out_stride=row, q_head_stride=512, q_out_head_stride=512, k=at + 2 * 48 * 256, k_stride=row,
+                v=at + 2 * 50 * 256, v_stride=row)
+    assert lib.limits_check_append(ctypes.byref(base.append_desc(c, b, **good))) == 0
+    for name, to in (("k", 47 * 256 - 8), ("v", 0), ("k", 256 * 46), ("v", 48 * 256 - 257 + 1), ("k", 49 * 256)):
+        inside = not set(_values(0, 3, row, 24, 512, 256)).isdisjoint(_values(to, 3, row, 2, 256, 256))          # rows repeat: three tell
+        status = lib.limits_check_append(ctypes.byref(base.append_desc(c, b, **{**good, name: at + 2 * to})))
+        assert status == (base.E_ALIAS if inside else 0), (name, to)
