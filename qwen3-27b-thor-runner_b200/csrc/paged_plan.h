@@ -250,6 +250,32 @@ inline bool rows_meet(const void* p, long long stride, long long heads, long lon
     if (stride == q_stride) return meet(d, {{stride, 1 - rows, rows - 1}, {head_stride, 0, heads - 1}, {q_head_stride, 1 - q_heads, 0}}, dim);
     return meet(d, {{stride, 0, rows - 1}, {q_stride, 1 - rows, 0}, {head_stride, 0, heads - 1}, {q_head_stride, 1 - q_heads, 0}}, dim);
 }
+// Whether two places of a tensor that is written, any two indices of its strides, share a value.  (Strides nested in any order, the usual case, are
+// told apart at once.)
+inline bool repeats(std::initializer_list<Steps> strides, int dim) {
+    Steps t[3];
+    int n = 0;
+    for (const Steps& x : strides) {                 // by rising stride
+        if (x.hi <= 0) continue;
+        int i = n++;
+        for (; i > 0 && t[i - 1].stride > x.stride; --i) t[i] = t[i - 1];
+        t[i] = x;
+    }
+    long long extent = dim;
+    bool nested = true;
+    for (int i = 0; i < n; ++i) {
+        nested = nested && t[i].stride >= extent;
+        extent += t[i].stride * t[i].hi;
+    }
+    if (nested) return false;
+    // two indices differ first in stride i, there by one or more
+    for (int i = 0; i < n; ++i) {
+        Steps u[3] = {{1, 0, 0}, {1, 0, 0}, {1, 0, 0}};
+        for (int j = i; j < n; ++j) u[j] = {t[j].stride, j == i ? 1 : -t[j].hi, t[j].hi};
+        if (meet(0, {u[0], u[1], u[2]}, dim)) return true;
+    }
+    return false;
+}
 // n steps of a stride stay far from the end of 64 bits
 inline bool fits(long long n, long long stride) { return n <= 0 || stride <= (1LL << 46) / n; }
 
@@ -333,9 +359,11 @@ inline int check_append(const nvfp4_kv_append_desc* d, AppendArgs* out, bool* em
     if (has_q) {
         if (int e = check_strides(a.q, a.q_stride, a.q_head, tokens, d->q_heads, dim)) return e;
         if (int e = check_strides(a.q_out, a.o_stride, a.o_head, tokens, d->q_heads, dim)) return e;
+        if (repeats({{a.o_stride, 0, tokens - 1}, {a.o_head, 0, d->q_heads - 1}}, dim)) return NVFP4_E_SHAPE;
     }
     if (int e = check_strides(a.k, a.k_stride, a.k_head, tokens, a.b.kv_heads, dim)) return e;
     if (int e = check_strides(a.v, a.v_stride, a.v_head, tokens, a.b.kv_heads, dim)) return e;
+    if (repeats({{a.b.page_stride, 0, a.b.num_pages - 1}, {a.b.token_stride, 0, a.b.page_size - 1}, {a.b.head_stride, 0, a.b.kv_heads - 1}}, dim)) return NVFP4_E_SHAPE;
     if (!aligned(d->q_norm, 16) || !aligned(d->k_norm, 16) || !aligned(d->inv_freq, 4) || !aligned(d->positions, 4)) return NVFP4_E_ALIGN;
     // in place: the same rows and heads, each read and written by the same thread
     const bool in_place = has_q && a.q == a.q_out && a.q_stride == a.o_stride && a.q_head == a.o_head;
@@ -380,6 +408,7 @@ inline int check_attention(const nvfp4_paged_attention_desc* d, AttentionArgs* o
     a.o_stride = d->out_stride; a.o_head = d->out_head_stride;
     if (int e = check_strides(a.q, a.q_stride, a.q_head, tokens, d->q_heads, dim)) return e;
     if (int e = check_strides(a.out, a.o_stride, a.o_head, tokens, d->q_heads, dim)) return e;
+    if (repeats({{a.o_stride, 0, tokens - 1}, {a.o_head, 0, d->q_heads - 1}}, dim)) return NVFP4_E_SHAPE;
     if (a.gate)
         if (int e = check_strides(a.gate, a.g_stride, a.g_head, tokens, d->q_heads, dim)) return e;
     const Span o = span_of(a.out, tokens, a.o_stride, d->q_heads, a.o_head, dim);

@@ -207,3 +207,39 @@ def test_keys_and_values_in_the_rows_of_queries_in_place(lib):
         inside = not set(_values(0, 3, row, 24, 512, 256)).isdisjoint(_values(to, 3, row, 2, 256, 256))          # rows repeat: three tell
         status = lib.limits_check_append(ctypes.byref(base.append_desc(c, b, **{**good, name: at + 2 * to})))
         assert status == (base.E_ALIAS if inside else 0), (name, to)
+
+
+def test_written_strides_that_repeat_a_place_are_refused(lib):
+    """Two heads or tokens in one place would be written by two threads: q_out, out and the cache of the append against the sets of their values' places."""
+    rng, dim, found = random.Random(9), 64, {"rows": [0, 0], "cache": [0, 0]}
+    steps = [64, 64, 72, 96, 128, 136, 192, 256, 320, 384, 512, 640, 1024]
+    for _ in range(2500):
+        rows, heads = rng.choice([1, 2, 3, 4, 7]), rng.choice([1, 2, 3, 5, 8])
+        stride, head = rng.choice(steps), rng.choice(steps)
+        places = _values(0, rows, stride, heads, head, dim)
+        want = base.E_SHAPE if len(set(places)) < len(places) else 0
+        c, b = base.cache(kv_heads=1, head_dim=dim, token_stride=64, page_stride=1024), base.batch(tokens=rows)
+        d = base.attention_desc(c, b, q_heads=heads, out_stride=stride, out_head_stride=head)
+        assert lib.limits_check_attention(ctypes.byref(d)) == want, (rows, heads, stride, head)
+        d = base.append_desc(c, b, q_heads=heads, rot_dim=0, q_out_stride=stride, q_out_head_stride=head)
+        assert lib.limits_check_append(ctypes.byref(d)) == want, (rows, heads, stride, head)
+        found["rows"][want != 0] += 1
+        # what is read may repeat: a cache with heads in common is attended to, not appended to
+        pages, page, kv_heads = rng.choice([1, 2, 3]), rng.choice([1, 2, 4]), rng.choice([1, 2, 3])
+        p, t, h = (rng.choice(steps) for _ in range(3))
+        places = [x + i * p for i in range(pages) for x in _values(0, page, t, kv_heads, h, dim)]
+        want = base.E_SHAPE if len(set(places)) < len(places) else 0
+        c = base.cache(num_pages=pages, page_size=page, kv_heads=kv_heads, head_dim=dim, page_stride=p, token_stride=t, head_stride=h)
+        b = base.batch(tokens=2)
+        assert lib.limits_check_append(ctypes.byref(base.append_desc(c, b, q_heads=2, rot_dim=0))) == want, (pages, page, kv_heads, p, t, h)
+        assert lib.limits_check_attention(ctypes.byref(base.attention_desc(c, b, q_heads=kv_heads))) == 0
+        found["cache"][want != 0] += 1
+    assert min(found["rows"] + found["cache"]) > 200
+    # large ones, in every order
+    big = dict(num_pages=1 << 20, page_size=256, kv_heads=8, head_dim=64)
+    for strides in [(256 * 512, 512, 64), (256 * 512, 64, 256 * 64), (64, (1 << 20) * 64, (1 << 28) * 64), (512, (1 << 20) * 512, 64)]:
+        names = dict(zip(("page_stride", "token_stride", "head_stride"), strides))
+        d = base.append_desc(base.cache(**big, **names, k=1 << 42, v=1 << 45), base.batch(), rot_dim=0)
+        assert lib.limits_check_append(ctypes.byref(d)) == 0
+        d = base.append_desc(base.cache(**big, **{**names, "token_stride": names["token_stride"] - 8}, k=1 << 42, v=1 << 45), base.batch(), rot_dim=0)
+        assert lib.limits_check_append(ctypes.byref(d)) == base.E_SHAPE
