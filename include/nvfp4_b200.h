@@ -362,7 +362,8 @@ typedef struct nvfp4_paged_batch {
  *          angle); positions [tokens] replaces the position as the angle's factor only (NULL: the token's own)
  * q may be NULL with q_heads = 0.  q_out may be q itself with q's strides (in place), and overlaps nothing else.  Head and token
  * strides in elements, multiples of 8, 0 = dense ([tokens][heads][head_dim]); k and v have the cache's heads.  What is written (q_out
- * and the cache here, out in the attention) has a place of its own for each head of each token: strides that repeat a place are refused.
+ * and the cache here, out in the attention) has a place of its own for each head of each token: strides that repeat a place are refused,
+ * and so are keys and values of the cache in one another's places.
  * All pointers on 16-byte boundaries (index arrays: 4).  A token of negative position (a padded sequence of kv_len 0) is left out; one
  * whose place is out of bounds writes its q_out only.  Two new tokens with the same place: one of them stays, no matter which. */
 typedef struct nvfp4_kv_append_desc {

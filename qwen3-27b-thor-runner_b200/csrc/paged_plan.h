@@ -370,6 +370,10 @@ inline int check_append(const nvfp4_kv_append_desc* d, AppendArgs* out, bool* em
     const Span q = span_of(a.q, tokens, a.q_stride, d->q_heads, a.q_head, dim), o = span_of(a.q_out, tokens, a.o_stride, d->q_heads, a.o_head, dim);
     const Span k = span_of(a.k, tokens, a.k_stride, a.b.kv_heads, a.k_head, dim), v = span_of(a.v, tokens, a.v_stride, a.b.kv_heads, a.v_head, dim);
     const Span ck = span_of_cache(a.b, a.b.k), cv = span_of_cache(a.b, a.b.v);
+    // keys and values may lie between one another (pages that hold both), but not in one another
+    if (ck.overlaps(cv) && meet(a.b.k - a.b.v, {{a.b.page_stride, 1 - a.b.num_pages, a.b.num_pages - 1}, {a.b.token_stride, 1 - a.b.page_size, a.b.page_size - 1},
+                                                  {a.b.head_stride, 1 - a.b.kv_heads, a.b.kv_heads - 1}}, dim))
+        return NVFP4_E_ALIAS;
     if (!in_place && (o.overlaps(q) || o.overlaps(k) || o.overlaps(v))) return NVFP4_E_ALIAS;
     // in place keys and values may lie between q's rows and heads, as a merged projection leaves them, but not in them
     if (in_place && o.overlaps(k) && rows_meet(a.q_out, a.o_stride, d->q_heads, a.o_head, a.k, a.k_stride, a.b.kv_heads, a.k_head, tokens, dim)) return NVFP4_E_ALIAS;

@@ -243,3 +243,23 @@ def test_written_strides_that_repeat_a_place_are_refused(lib):
         assert lib.limits_check_append(ctypes.byref(d)) == 0
         d = base.append_desc(base.cache(**big, **{**names, "token_stride": names["token_stride"] - 8}, k=1 << 42, v=1 << 45), base.batch(), rot_dim=0)
         assert lib.limits_check_append(ctypes.byref(d)) == base.E_SHAPE
+
+
+def test_keys_and_values_of_the_cache_in_one_another(lib):
+    """Pages that hold both, in any order, are appended to; a value in a key's place is refused.  Attention, which only reads, takes one tensor for both."""
+    rng, dim, found = random.Random(10), 64, [0, 0]
+    at = 1 << 30
+    for _ in range(1500):
+        pages, page, kv_heads = rng.choice([1, 2, 3]), rng.choice([1, 2, 4]), rng.choice([1, 2, 3])
+        h = rng.choice([64, 128, 136])
+        t = h * kv_heads * rng.choice([1, 2])
+        p = t * page * rng.choice([1, 2]) + rng.choice([0, 64])
+        off = 8 * rng.randint(-5, pages * p // 8 + 5) if rng.random() < 0.5 else rng.choice([64, h * kv_heads, t * page, pages * p, -64, 0])
+        keys = [x + i * p for i in range(pages) for x in _values(0, page, t, kv_heads, h, dim)]
+        want = not set(keys).isdisjoint(x + off for x in keys)
+        c = base.cache(k=at, v=at + 2 * off, num_pages=pages, page_size=page, kv_heads=kv_heads, head_dim=dim, page_stride=p, token_stride=t, head_stride=h)
+        b = base.batch(tokens=2)
+        assert lib.limits_check_append(ctypes.byref(base.append_desc(c, b, q_heads=2, rot_dim=0))) == (base.E_ALIAS if want else 0), (pages, page, kv_heads, p, t, h, off)
+        assert lib.limits_check_attention(ctypes.byref(base.attention_desc(c, b, q_heads=kv_heads))) == 0
+        found[want] += 1
+    assert min(found) > 200
