@@ -445,7 +445,7 @@ int nvfp4_linear_host(nvfp4_handle* h, const void* A_host, int M,
  * 0 = no kernel of this handle ever gave up a bounded wait; otherwise the code of the first
  * wait that ran out (0x1xx producer ring slot, 0x2xx consumer ring slot, 0x300 cross-CTA
  * partial flag, 0x4xx tensor-core pipeline, 0xA10 a ring slot and 0xA2x to 0xA4x the pipeline of
- * nvfp4_paged_attention), or 0xA01: a place out of bounds in a paged cache was left out. */
+ * nvfp4_paged_attention), or, while no wait has run out, 0xA01: a place out of bounds in a paged cache was left out. */
 int nvfp4_device_status(nvfp4_handle* h, unsigned int* status);
 
 /* Number of kernels this library has launched on the handle since creation. */

@@ -34,6 +34,7 @@ struct nvfp4_handle {
     int gemm_weight_rounding = 0;                // above 8 tokens: the reference's BF16-rounded weights (its GEMM branch)
     unsigned long long launches = 0;
     char* paged_scratch = nullptr;               // parts of split sequences in nvfp4_paged_attention (44 MB on 148 SMs)
+    unsigned int* paged_places = nullptr;        // behind them: whether a place out of bounds was left out
     int host_direct_out = 1;                     // nvfp4_linear_host: kernels store into a pinned, device-mapped C_host themselves
     // scale tensors in which nvfp4_scan_scales found a byte 0x7F / 0xFF: the tensor core reads those as NaN, so
     // these weights stay on the kernels that decode the scale themselves
@@ -297,8 +298,9 @@ int nvfp4_create(int device, size_t workspace_bytes, nvfp4_handle** out) {
     e = cudaMalloc(&h->workspace, workspace_bytes);
     if (e == cudaSuccess) e = cudaMemset(h->workspace, 0, workspace_bytes);
     const size_t paged_bytes = paged_scratch_bytes(h->dev.sm_count) + paged_prefill_scratch_bytes(h->dev.sm_count);
-    if (e == cudaSuccess) e = cudaMalloc(&h->paged_scratch, paged_bytes);
-    if (e == cudaSuccess) e = cudaMemset(h->paged_scratch, 0, paged_bytes);
+    if (e == cudaSuccess) e = cudaMalloc(&h->paged_scratch, paged_bytes + sizeof(unsigned int));
+    if (e == cudaSuccess) e = cudaMemset(h->paged_scratch, 0, paged_bytes + sizeof(unsigned int));
+    h->paged_places = reinterpret_cast<unsigned int*>(h->paged_scratch + paged_bytes);
     if (e == cudaSuccess) e = configure_kernels(h->dev);
     cudaSetDevice(prev);
     if (e != cudaSuccess) {
@@ -404,7 +406,10 @@ int nvfp4_device_status(nvfp4_handle* h, unsigned int* status) {
     cudaGetDevice(&prev);
     cudaSetDevice(h->dev.device);
     cudaError_t e = cudaDeviceSynchronize();
-    if (e == cudaSuccess) e = cudaMemcpy(status, h->workspace, sizeof(unsigned int), cudaMemcpyDeviceToHost);
+    unsigned int wait = 0, place = 0;
+    if (e == cudaSuccess) e = cudaMemcpy(&wait, h->workspace, sizeof(unsigned int), cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess) e = cudaMemcpy(&place, h->paged_places, sizeof(unsigned int), cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess) *status = paged::reported(wait, place);
     cudaSetDevice(prev);
     return cuda_status(e);
 }
@@ -768,6 +773,7 @@ int nvfp4_kv_append(nvfp4_handle* h, const nvfp4_kv_append_desc* d, nvfp4_stream
     if (int e = paged::check_append(d, &a, &empty)) return e;
     if (empty) return NVFP4_OK;
     a.b.status = reinterpret_cast<unsigned int*>(h->workspace);
+    a.b.places = h->paged_places;
     OnDevice on(h->dev.device);
     if (on.e != cudaSuccess) return (int)on.e;
     int nl = 0;
@@ -783,6 +789,7 @@ int nvfp4_paged_attention(nvfp4_handle* h, const nvfp4_paged_attention_desc* d, 
     if (int e = paged::check_attention(d, &a, &empty)) return e;
     if (empty) return NVFP4_OK;
     a.b.status = reinterpret_cast<unsigned int*>(h->workspace);
+    a.b.places = h->paged_places;
     OnDevice on(h->dev.device);
     if (on.e != cudaSuccess) return (int)on.e;
     // 16 rows (new tokens x heads of a group) of a sequence share a tile of the few-token kernel, which runs at the rate of the cache's bytes, read once for

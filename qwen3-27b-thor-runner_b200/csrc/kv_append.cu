@@ -102,7 +102,7 @@ kv_append_kernel(AppendArgs a, int per) {
     begin_head();
     ask(0);
     // cu_q ascends: its ends tell whether rows outside [0, tokens] are left out
-    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == kThreads - 1 && b.cu_q && (b.cu_q[0] < 0 || b.cu_q[b.sequences] > b.tokens)) atomicCAS(b.status, 0u, kStatusPlace);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && tid == kThreads - 1 && b.cu_q && (b.cu_q[0] < 0 || b.cu_q[b.sequences] > b.tokens)) *b.places = kStatusPlace;
     if (warp < tokens) {
         int seq, pos = 0;
         const bool there = find_row(b, t0 + warp, seq, pos);
@@ -111,7 +111,7 @@ kv_append_kernel(AppendArgs a, int per) {
         if (there && pos < b.max_kv) at = place(b, seq, pos);
         if ((tid & 31) == 0) {
             s_at[warp] = at;
-            if (at == -1) atomicCAS(b.status, 0u, kStatusPlace);
+            if (at == -1) *b.places = kStatusPlace;
         }
         for (int i = tid & 31; i < half; i += 32) {
             double angle = (double)p * (double)a.inv_freq[i];

@@ -207,7 +207,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         at.n = Cursor<D>::items(p, at.q);
         mine += (long long)at.n.items * at.n.cost();
         // one block says so, the one that is the last to have work of its own
-        if (blockIdx.x + 1 == gridDim.x && cut_off(b, s)) atomicCAS(b.status, 0u, kStatusPlace);
+        if (blockIdx.x + 1 == gridDim.x && cut_off(b, s)) *b.places = kStatusPlace;
     }
     long long upto = mine;
 #pragma unroll
@@ -269,7 +269,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     auto load = [&](int stage) {
         if (ld_more) {
             const bool there = seen_ahead && (unsigned)page_ahead < (unsigned)b.num_pages;
-            if (seen_ahead && !there) atomicCAS(b.status, 0u, kStatusPlace);
+            if (seen_ahead && !there) *b.places = kStatusPlace;
             unsigned int ok = __ballot_sync(0xffffffffu, there);
             unsigned char* ks = ring + stage * F::kStageBytes;
             unsigned char* vs = ks + F::kHalfStage;

@@ -17,6 +17,8 @@ namespace nvfp4 {
 namespace paged {
 
 constexpr unsigned int kStatusPlace = 0xA01u;      // a page number or position out of bounds was left out
+// What a handle reports: a wait that ran out, whose results are worth nothing, before a place that was left out.
+inline unsigned int reported(unsigned int wait, unsigned int place) { return wait ? wait : place; }
 constexpr int kMaxPositions = 0x7fffffff - 65536;  // positions are 32-bit numbers, with room for a tile behind the last one
 
 template <class T>
@@ -47,7 +49,8 @@ struct Batch {
     long long page_stride, token_stride, head_stride;
     int max_kv;                        // table_cols * page_size
     PageDivider div;
-    unsigned int* status;              // the handle's status word
+    unsigned int* status;              // the handle's status word: the first wait that ran out
+    unsigned int* places;              // and its word for places out of bounds, so that these hide no wait
 };
 
 struct Sequence {
@@ -307,7 +310,7 @@ inline int check_batch(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, Batc
     }
     *out = Batch{b->cu_q, b->kv_len, b->block_table, b->table_stride, b->table_cols, b->sequences, b->tokens, b->max_q_len,
                  static_cast<uint16_t*>(c->k), static_cast<uint16_t*>(c->v), c->num_pages, c->page_size, c->kv_heads, c->head_dim,
-                 c->page_stride, c->token_stride, c->head_stride, b->table_cols * c->page_size, make_divider(c->page_size), nullptr};
+                 c->page_stride, c->token_stride, c->head_stride, b->table_cols * c->page_size, make_divider(c->page_size), nullptr, nullptr};
     return NVFP4_OK;
 }
 inline Span span_of_cache(const Batch& b, const void* p) {

@@ -334,7 +334,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
         const LongItems n = Cursor<D>::items(p, q);
         mine += long_places(q, n, n.tiles) * n.heads;
         // one block says so, the one that is the last to have work of its own
-        if (blockIdx.x + 1 == gridDim.x && cut_off(b, s)) atomicCAS(b.status, 0u, kStatusPlace);
+        if (blockIdx.x + 1 == gridDim.x && cut_off(b, s)) *b.places = kStatusPlace;
     }
     long long upto = mine;
 #pragma unroll
@@ -424,7 +424,7 @@ paged_prefill_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_const
                 place = tok - entry * b.page_size;
                 page = b.table[(long long)at.s * b.table_stride + entry];
                 if ((unsigned)page >= (unsigned)b.num_pages) {
-                    atomicCAS(b.status, 0u, kStatusPlace);
+                    *b.places = kStatusPlace;
                     page = -1;
                 }
             }

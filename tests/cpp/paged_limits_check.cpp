@@ -11,6 +11,7 @@ int paged_cut_off(const nvfp4_kv_cache* c, const nvfp4_paged_batch* b, int s) {
     return check_batch(c, b, &x) ? -1 : cut_off(x, s);
 }
 
+unsigned int limits_reported(unsigned int wait, unsigned int place) { return reported(wait, place); }
 int limits_check_append(const nvfp4_kv_append_desc* d) {
     AppendArgs a{};
     bool empty = false;

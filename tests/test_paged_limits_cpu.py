@@ -263,3 +263,14 @@ def test_keys_and_values_of_the_cache_in_one_another(lib):
         assert lib.limits_check_attention(ctypes.byref(base.attention_desc(c, b, q_heads=kv_heads))) == 0
         found[want] += 1
     assert min(found) > 200
+
+
+def test_a_place_left_out_hides_no_wait_that_ran_out(lib):
+    """Results behind a wait that ran out are worth nothing; a page number out of bounds, whenever it was found, is told only while there is no such wait."""
+    assert [lib.limits_reported(w, p) for w, p in [(0, 0), (0, 0xA01), (0x701, 0), (0x701, 0xA01), (0xA10, 0xA01)]] == [0, 0xA01, 0x701, 0x701, 0xA10]
+    csrc = os.path.join(ROOT, "qwen3-27b-thor-runner_b200", "csrc")
+    for name in sorted(os.listdir(csrc)):
+        if name.endswith((".cu", ".cuh", ".h")):
+            text = open(os.path.join(csrc, name)).read()
+            for line in [x for x in text.split("\n") if "kStatusPlace" in x and "constexpr" not in x]:
+                assert "places = kStatusPlace;" in line, (name, line)
