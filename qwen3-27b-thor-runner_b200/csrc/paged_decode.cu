@@ -366,7 +366,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     int from = at.chunk;                             // the first unit of the item that is this block's
     while (more) {
         if (TMA) {
-            ptx::mbar_wait(&full[stage], parity, s_abort, b.status, 0xA10u);
+            // run out: nothing more is asked for; the warp goes on through its units, whose results are worth nothing, so that no other waits for it
+            if (!__all_sync(0xffffffffu, ptx::mbar_wait(&full[stage], parity, s_abort, b.status, 0xA10u))) ld_more = false;
         } else {
             cp_async_wait<F::kStages - 2>();
         }
@@ -600,6 +601,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         clear();
     }
     if (!TMA) cp_async_wait<0>();
+    if (TMA && *reinterpret_cast<volatile int*>(s_abort)) {            // loads may still be on their way into this block's shared memory
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
+    }
 }
 
 // Adds the parts of split items in the order of their blocks.  A kernel of its own behind the other one: there the last block to arrive would

@@ -63,3 +63,15 @@ def test_no_wait_of_the_prompt_kernel_spans_a_run():
     assert src.count("mbar_wait(&drain[") == 1
     kernel = src[src.index("paged_prefill_kernel("):at]
     assert kernel.rfind("__syncthreads();") > kernel.rfind("more = at.next_item(")
+
+
+def test_few_token_attention_stops_loading_behind_a_wait_that_ran_out():
+    """No load is issued into a ring whose waits have given up, and a block does not end while one may be on its way into its shared memory."""
+    src = source("paged_decode.cu")
+    kernel = src[src.index("paged_decode_kernel("):src.index("paged_join_kernel(")]
+    assert re.findall(r"[^;]*mbar_wait\([^;]*;", kernel) and all(re.search(r"if \(!__all_sync\(0xffffffffu, ptx::mbar_wait\([^;]*\)\) ld_more = false;", w)
+                                                                for w in re.findall(r"[^;{]*mbar_wait\([^;]*;", kernel))
+    body = kernel[kernel.index("auto load = [&](int stage)"):]
+    assert body.index("if (ld_more) {") < body.index("tma_load_5d(")
+    end = kernel[kernel.index("clear();\n    }"):] if "clear();\n    }" in kernel else kernel[kernel.rindex("clear();"):]
+    assert re.search(r"if \(TMA && \*reinterpret_cast<volatile int\*>\(s_abort\)\) \{\s*for \([^)]*\) __nanosleep", end)
