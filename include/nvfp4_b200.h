@@ -384,12 +384,13 @@ typedef struct nvfp4_kv_append_desc {
 int nvfp4_kv_append(nvfp4_handle* h, const nvfp4_kv_append_desc* desc, nvfp4_stream_t stream);
 
 /* out[r, h] = bf16( sum_j softmax_j(scale * q[r, h] . k[j, h / g]) v[j, h / g]  (* sigmoid(gate[r, h])) ) over the positions j up to
- * the row's own of its sequence's pages, g = q_heads / kv_heads; FP32 scores, maxima and sums, weights rounded to BF16 for the
- * product with v.  A row that sees no key gives zeros.  scale 0 = 1 / sqrt(head_dim).  The keys and values of the new tokens must be in
- * the cache (nvfp4_kv_append in front, on the same stream).  Slots behind a sequence's last token may hold anything, infinities and
- * NaN included; a NaN or infinity in a value of the sequence itself reaches the rows that see it and may reach rows in front of it in
- * the same call.  One token per sequence, a few (verification of drafted tokens), prompts and mixtures of them; work is split over the
- * lengths found on the device and joined in a fixed order, so a result depends on the batch and its bounds, not on timing.
+ * the row's own of its sequence's pages, g = q_heads / kv_heads; FP32 scores, maxima and sums.  Sequences of few new tokens (max_q_len * g
+ * up to 32, or in a mixed batch that many rows of the sequence) have one rounding, the result's; in others the weights too are rounded to
+ * BF16 for the product with v (errors of 0.0022 instead of 0.0017 of the result's norm).  A row that sees no key gives zeros.
+ * scale 0 = 1 / sqrt(head_dim).  The keys and values of the new tokens must be in the cache (nvfp4_kv_append in front, on the same stream).
+ * Slots behind a sequence's last token may hold anything, infinities and NaN included; a NaN or infinity in a value of the sequence
+ * itself reaches the rows that see it (an infinity perhaps as NaN) and may reach rows in front of it in the same call.  One token per sequence, a few (verification of drafted tokens), prompts and mixtures of them; work is split over the lengths
+ * found on the device and joined in a fixed order, so a result depends on the batch and its bounds, not on timing.
  * Strides, alignment and defaults as above; out overlaps neither q, gate nor the cache.  Uses a scratch that belongs to the handle. */
 typedef struct nvfp4_paged_attention_desc {
     const nvfp4_kv_cache* cache;

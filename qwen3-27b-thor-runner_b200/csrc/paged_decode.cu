@@ -13,9 +13,12 @@
 //    maximum and sum of its own: no barrier between warps inside an item, two stages always under way (128 KB of loads in flight on an SM), and
 //    the loads run on across the borders of items.  Pages that are no multiple of eight tokens come by cp.async, 16 bytes a thread (at pages of 16
 //    and 32 tokens nearly as fast: 64 sequences, heads of 256, TMA 83, cp.async 82 us; 243 sequences, heads of 128, 109 and 111).
-//  * Scores, maxima, sums and results stay in registers.  The weights 2^(t - m) are rounded to BF16 as the MMA's operand (2^-9 relative
-//    to each, below the rounding of the result); the sums take them unrounded in FP32.  The maximum follows only when a score passes it by 8
-//    (weights up to 2^8), which spares nearly every rescaling of the results.
+//  * Scores, maxima, sums and results stay in registers.  The weights 2^(t - m) enter the second product as two BF16 operands, the rounded weight and
+//    what its rounding left (2^-16 of it is lost): one operand alone would be off by up to 2^-8, as much as the result's own rounding (error against 64
+//    bits 0.0022 instead of 0.0017).  With up to eight rows in a tile the second operand lies in the places of the other eight rows and costs
+//    nothing on the tensor core, otherwise the product is done twice; 64 sequences, 12 rows of 256: 84.3 us with one operand, 85.7 with two; 243 sequences, 4 rows of
+//    128: 110.8, 112.2.  The sums take the weights unrounded in FP32.  The maximum follows only when a score passes it by 8 (weights up to 2^8), which spares
+//    nearly every rescaling of the results.
 //  * At an item's end the warps' results are added in shared memory in warp order.  Parts of a split item go to the handle's scratch and are added
 //    in block order by a second kernel.
 // Measured: 64 sequences of 128 to 16384 tokens, 24 heads over 2 of 256, 84 us, 0.77 of the copy rate in cache bytes; 243 sequences, 32 heads over 8 of 128,
@@ -364,6 +367,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
     begin_item();
     clear();
     int from = at.chunk;                             // the first unit of the item that is this block's
+    bool low = at.q.q_len * a.group - at.tile * kRows <= 8;      // the tile's rows are the first eight at most
     while (more) {
         if (TMA) {
             // run out: nothing more is asked for; the warp goes on through its units, whose results are worth nothing, so that no other waits for it
@@ -439,7 +443,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
             g1 = fmaxf(g1, __shfl_xor_sync(0xffffffffu, g1, 2));
             if (__any_sync(0xffffffffu, g0 > m0 + 8.0f || g1 > m1 + 8.0f)) {
                 const float n0 = fmaxf(m0, g0), n1 = fmaxf(m1, g1);
-                const float c0 = n0 == m0 ? 1.0f : ex2(m0 - n0), c1 = n1 == m1 ? 1.0f : ex2(m1 - n1);
+                const float c0 = n0 == m0 ? 1.0f : ex2(m0 - n0), c1 = low ? c0 : n1 == m1 ? 1.0f : ex2(m1 - n1);
                 m0 = n0;
                 m1 = n1;
                 l0 *= c0;
@@ -453,27 +457,38 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
                 }
             }
             const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                t[n][0] = ex2(t[n][0] - b0);
-                t[n][1] = ex2(t[n][1] - b0);
-                t[n][2] = ex2(t[n][2] - b1);
-                t[n][3] = ex2(t[n][3] - b1);
-                l0 += t[n][0] + t[n][1];
-                l1 += t[n][2] + t[n][3];
-            }
-            const uint32_t pf[4] = {pack_bf16(t[0][0], t[0][1]), pack_bf16(t[0][2], t[0][3]), pack_bf16(t[1][0], t[1][1]), pack_bf16(t[1][2], t[1][3])};
             const int tok = lane & 15;
             uint32_t off[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) off[i] = vs + tok * 128 + (((i * 2 + (lane >> 4)) ^ (tok & 7)) << 4);
+            // The weights are two BF16 operands, the rounded ones and what their rounding left, which lies in the places of rows 8 to 15 where the
+            // tile has none.
+            auto multiply = [&](auto halves) {
+                constexpr int kRowHalves = decltype(halves)::value;          // 1: rows 0 to 7 only
+                uint32_t w[2][4];
 #pragma unroll
-            for (int c = 0; c < F::kTiles; c += 2) {
-                uint32_t r[4];
-                ldmatrix_x4_trans(r, off[c / 2 & 3] + (c >> 3) * (kGroup * 128));
-                ptx::mma_bf16_16x8x16(o[c], pf, r[0], r[1]);
-                ptx::mma_bf16_16x8x16(o[c + 1], pf, r[2], r[3]);
-            }
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int h = 0; h < kRowHalves; ++h) {
+                        const float x = ex2(t[n][2 * h] - (h ? b1 : b0)), y = ex2(t[n][2 * h + 1] - (h ? b1 : b0));
+                        (h ? l1 : l0) += x + y;
+                        const uint32_t rounded = pack_bf16(x, y);
+                        w[0][2 * n + h] = rounded;
+                        w[kRowHalves - 1][2 * n + h + 2 - kRowHalves] = pack_bf16(x - __uint_as_float(rounded << 16), y - __uint_as_float(rounded & 0xFFFF0000u));
+                    }
+#pragma unroll
+                for (int c = 0; c < F::kTiles; c += 2) {
+                    uint32_t r[4];
+                    ldmatrix_x4_trans(r, off[c / 2 & 3] + (c >> 3) * (kGroup * 128));
+#pragma unroll
+                    for (int i = 0; i < kRowHalves; ++i) {
+                        ptx::mma_bf16_16x8x16(o[c], w[i], r[0], r[1]);
+                        ptx::mma_bf16_16x8x16(o[c + 1], w[i], r[2], r[3]);
+                    }
+                }
+            };
+            if (low) multiply(std::integral_constant<int, 1>{});
+            else multiply(std::integral_constant<int, 2>{});
         }
         if (++stage == F::kStages) {
             stage = 0;
@@ -524,7 +539,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
 #pragma unroll
                 for (int i = 0; i < kRoundTiles; ++i) {
                     const float(&x)[4] = o[rd * kRoundTiles + i];
-                    if (kLow) merge2[(warp * kRoundTiles + i) * 32 + lane] = make_float2(x[0], x[1]);
+                    if (kLow) merge2[(warp * kRoundTiles + i) * 32 + lane] = make_float2(x[0] + x[2], x[1] + x[3]);
                     else merge[(warp * kRoundTiles + i) * 32 + lane] = make_float4(x[0], x[1], x[2], x[3]);
                 }
                 if (rd == 0 && col0 == 0 && (lane & 3) == 0) {
@@ -599,6 +614,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
         }
         if (F::kHalves == 2) __syncthreads();        // the next item's scores go where the results were added
         clear();
+        low = at.q.q_len * a.group - at.tile * kRows <= 8;
     }
     if (!TMA) cp_async_wait<0>();
     if (TMA && *reinterpret_cast<volatile int*>(s_abort)) {            // loads may still be on their way into this block's shared memory

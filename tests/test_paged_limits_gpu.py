@@ -85,3 +85,37 @@ def test_rows_outside_the_batch_are_told(starts, call):
     run()
     assert h.device_status() == 0xA01
     h.close()
+
+
+@pytest.mark.parametrize("dim,q_heads,kv_heads,new,past", [
+    (128, 32, 8, [1] * 5, [0, 1, 40, 700, 3000]), (128, 16, 1, [1, 1], [900, 60]), (256, 24, 2, [1, 1, 1], [5, 333, 5000]), (256, 8, 1, [1, 1], [1500, 64]),
+    (64, 7, 1, [1, 2, 3, 4], [50, 0, 900, 20]), (64, 24, 3, [3, 1], [128, 2000]), (256, 6, 1, [4, 1, 2], [100, 900, 2]), (128, 8, 2, [1], [40000])])
+@pytest.mark.parametrize("page", [16, 5])
+def test_few_tokens_round_the_result_only(dim, q_heads, kv_heads, new, past, page):
+    """One rounding to BF16, that of the result.  Queries and keys are multiples of 1/4 up to 2, so that their products are exact and what is left is: a weight's two
+    operands, off by 2^-16 of it; exp2 and its argument, 2^-20 and the score's own 2^-22; the tensor core's and the sums' 2^-22 of what is there for each 16 keys
+    and for 64 additions at the end."""
+    h = nvfp4.Handle(0, 16 << 20)
+    c = ref.Case(new, past, q_heads, kv_heads, dim, page, seed=dim + q_heads)
+    g = torch.Generator(device="cuda").manual_seed(dim + page)
+    quarters = lambda x: x.copy_(torch.randint(-8, 9, x.shape, device="cuda", generator=g) / 4)
+    quarters(c.q), quarters(c.k_cache)
+    cache, batch = c.objects(nvfp4)
+    h.paged_attention(cache, batch, c.q, c.out)
+    torch.cuda.synchronize()
+    worst = 0.0
+    for s, (n, kv) in enumerate(zip(c.new, c.kv)):
+        rows = slice(int(c.starts[s]), int(c.starts[s]) + n)
+        k, v = c.keys(c.k_cache, s, kv), c.keys(c.v_cache, s, kv)
+        hidden = torch.arange(kv, device="cuda")[None, :] > torch.arange(kv - n, kv, device="cuda")[:, None]
+        for hd in range(q_heads):
+            t = (c.q[rows, hd].double() @ k[:, hd * kv_heads // q_heads].T * dim ** -0.5).masked_fill(hidden, -float("inf"))
+            w = torch.softmax(t, -1)
+            o, a = w @ v[:, hd * kv_heads // q_heads], w @ v[:, hd * kv_heads // q_heads].abs()
+            score = t.masked_fill(hidden, 0.0).abs().amax(-1, keepdim=True)
+            rel = 2.0 ** -16 + 2.0 ** -20 + (2 * score + kv / 16 + 64) * 2.0 ** -22
+            tol = rel * a * (1 + ref.BF16_HALF_STEP) + ref.BF16_HALF_STEP * o.abs() + 1e-30
+            worst = max(worst, float(((c.out[rows, hd].double() - o).abs() / tol).max()))
+    assert worst <= 1.0
+    assert h.device_status() == 0
+    h.close()
