@@ -1,4 +1,5 @@
 """The paged cache's calls at the ends of what they take: runs longer than a wait's limit, lengths and offsets out of bounds."""
+import numpy as np
 import pytest
 import torch
 
@@ -117,5 +118,84 @@ def test_few_tokens_round_the_result_only(dim, q_heads, kv_heads, new, past, pag
             tol = rel * a * (1 + ref.BF16_HALF_STEP) + ref.BF16_HALF_STEP * o.abs() + 1e-30
             worst = max(worst, float(((c.out[rows, hd].double() - o).abs() / tol).max()))
     assert worst <= 1.0
+    assert h.device_status() == 0
+    h.close()
+
+
+def _plant(c, seed):
+    """Every query is aligned with two keys that it sees, which share its attention: a key left out, or counted twice, changes its result by a sixth of a value and more.
+    The two lie at positions spread over all that the row sees, its first, its last and those around multiples of 16 among them."""
+    rng = np.random.default_rng(seed)
+    sign = torch.Generator(device="cuda").manual_seed(seed)
+    c.k_cache.copy_(torch.randint(0, 2, c.k_cache.shape, device="cuda", generator=sign) * 2 - 1)
+    g = c.q_heads // c.kv_heads
+    for s, (n, kv) in enumerate(zip(c.new, c.kv)):
+        if n == 0:
+            continue
+        keys = c.keys(c.k_cache, s, kv)
+        see = np.arange(kv - n, kv)[:, None] + 1
+        at = [(rng.random((n, c.q_heads)) * see).astype(np.int64) for _ in range(2)]
+        edges = rng.integers(0, 4, (n, c.q_heads))
+        near = np.clip(at[0] // 16 * 16 + rng.integers(-1, 2, at[0].shape), 0, see - 1)
+        at[0] = np.choose(edges, [at[0], near, np.broadcast_to(see - 1, at[0].shape), np.zeros_like(at[0])])
+        heads = torch.arange(c.q_heads, device="cuda")[None, :] // g
+        both = sum(keys[torch.from_numpy(p).cuda(), heads] for p in at)
+        c.q[int(c.starts[s]):int(c.starts[s]) + n] = both * (2.0 if c.dim > 64 else 4.0)
+
+
+@pytest.mark.parametrize("dim,q_heads,kv_heads", [(256, 24, 2), (128, 8, 8), (128, 32, 8), (64, 20, 1)])
+@pytest.mark.parametrize("page", [16, 24, 7])
+def test_every_key_counts_once_in_decode(dim, q_heads, kv_heads, page):
+    h = nvfp4.Handle(0, 16 << 20)
+    for seed, past in enumerate([[4999], [17] * 3 + [2000, 63, 64, 65, 130, 999], list(range(100, 3100, 53))]):
+        c = ref.Case([1] * len(past), past, q_heads, kv_heads, dim, page, seed=seed)
+        for turn in range(6 if len(past) == 1 else 1):
+            _plant(c, 10 * seed + turn)
+            cache, batch = c.objects(nvfp4)
+            want, tol = ref.attention(c)
+            h.paged_attention(cache, batch, c.q, c.out)
+            torch.cuda.synchronize()
+            assert ref.worst(c.out, want, tol) <= 1.0, (seed, turn)
+    assert h.device_status() == 0
+    h.close()
+
+
+@pytest.mark.parametrize("dim,q_heads,kv_heads,new,past", [
+    (256, 24, 2, [700], [1300]), (256, 4, 4, [129, 1, 300, 2], [1, 900, 511, 40]), (128, 32, 8, [260, 1, 40], [0, 700, 2000]), (128, 6, 2, [1000], [3000]),
+    (64, 12, 6, [513, 3], [255, 800]), (64, 5, 1, [128, 128, 128], [0, 128, 129])])
+@pytest.mark.parametrize("page", [16, 64, 24])
+def test_every_key_counts_once_in_prompts(dim, q_heads, kv_heads, new, past, page):
+    h = nvfp4.Handle(0, 16 << 20)
+    c = ref.Case(new, past, q_heads, kv_heads, dim, page, seed=dim + page, pad=1)
+    _plant(c, dim + page)
+    cache, batch = c.objects(nvfp4)
+    want, tol = ref.attention(c)
+    h.paged_attention(cache, batch, c.q, c.out)
+    torch.cuda.synchronize()
+    assert ref.worst(c.out, want, tol) <= 1.0 and h.device_status() == 0
+    h.close()
+
+
+@pytest.mark.parametrize("dim,q_heads,kv_heads", [(256, 12, 2), (128, 8, 2), (64, 6, 6)])
+@pytest.mark.parametrize("new,past", [([1] * 7, [0, 15, 16, 90, 300, 1000, 2000]), ([150, 1, 33, 4], [10, 500, 0, 77])])
+def test_rows_head_by_head(dim, q_heads, kv_heads, new, past):
+    """[heads][tokens][dim]: the head's stride above the token's, for queries, gates, new keys and values and the results."""
+    h = nvfp4.Handle(0, 16 << 20)
+    c = ref.Case(new, past, q_heads, kv_heads, dim, 16, seed=dim, gate=True, pad=3)
+    swap = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)
+    for name in ("q", "gate", "k", "v", "out"):
+        setattr(c, name, swap(getattr(c, name)))
+    assert c.q.stride(1) > c.q.stride(0)
+    cache, batch = c.objects(nvfp4)
+    want, tol = ref.attention(c)
+    h.paged_attention(cache, batch, c.q, c.out, gate=c.gate)
+    torch.cuda.synchronize()
+    assert ref.worst(c.out, want, tol) <= 1.0
+    c.out.fill_(7.0)
+    f = (1e4 ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)).float().cuda()
+    (want_q, q_tol), (want_k, k_tol), want_v = ref.append(c, None, None, 1e-6, f)
+    h.kv_append(cache, batch, c.q, c.k, c.v, c.out, inv_freq=f)
+    torch.cuda.synchronize()
+    assert ref.worst(c.out, want_q, q_tol) <= 1.0 and ref.worst(c.k_cache, want_k, k_tol) <= 1.0 and torch.equal(c.v_cache.double(), want_v)
     assert h.device_status() == 0
     h.close()
