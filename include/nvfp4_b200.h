@@ -340,7 +340,8 @@ typedef struct nvfp4_kv_cache {
  * new tokens.  Position p of sequence s lies in slot p % page_size of page block_table[s * table_stride + p / page_size].
  * cu_q, kv_len and block_table are DEVICE memory and follow the stream like the data, so a captured call may be replayed with
  * other contents; tokens, sequences, table_cols and max_q_len are the host's bounds and stay as captured.
- *   tokens     rows of q, k, v and out.  Rows behind cu_q[sequences] (a padded batch) are neither read nor written.
+ *   tokens     rows of q, k, v and out.  Rows behind cu_q[sequences] (a padded batch) are not written; they may be read, and what they
+ *              hold does not matter.
  *   max_q_len  the longest run of new tokens to be expected; it selects kernels, a longer run is slower, not wrong.
  * Entries of a table row behind the sequence's last page are not used.  What the device finds out of bounds is left out, and
  * nvfp4_device_status says so (0xA01): a page number outside [0, num_pages) or a position behind table_cols pages takes part in

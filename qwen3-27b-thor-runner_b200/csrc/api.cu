@@ -795,7 +795,8 @@ int nvfp4_paged_attention(nvfp4_handle* h, const nvfp4_paged_attention_desc* d, 
     // 16 rows (new tokens x heads of a group) of a sequence share a tile of the few-token kernel, which runs at the rate of the cache's bytes, read once for
     // each tile; a tcgen05 tile holds 128, and a pair of SMs two to four.  Measured, few-token kernel and the other, us: 32 sequences of 8 tokens x 4 heads
     // of 128 (32 rows) 131, 199; 24 of 4 x 8 of 64 (32) 31, 54; 64 of 4 x 6 of 256 (24) 178, 163; 16 of 8 x 6 of 256 (48) 86, 67; 12 of 4 x 12 of 256
-    // (48) 42, 41; 32 of 16 x 4 of 128 (64) 242, 199.  Two tiles it is.  (Both in one pass over the cache, a head shared by twice as many warps, won
+    // (48) 42, 41; 32 of 16 x 4 of 128 (64) 242, 199.  (The few-token kernel's figures with one operand of weights; two add up to 4 %: 183 for 178.)  Two tiles
+    // it is, for all head sizes, though heads of 256 would turn at one.  (Both in one pass over the cache, a head shared by twice as many warps, won
     // nothing: they meet and form the same weights more often; 187 for 178, 130 for 131.)  The host knows bounds only: where they leave no room for
     // sequences of both kinds, one kernel takes all, otherwise each takes its own.
     constexpr int kFewRows = 2 * paged::kRows;

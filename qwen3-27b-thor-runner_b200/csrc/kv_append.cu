@@ -1,12 +1,12 @@
 // New tokens into the paged cache: norms of queries and keys for each head, rotation by the position, and the writes of keys and
 // values to their places, in one pass (the reference's fused qk-norm-rope and KV-write kernels, src/engine/light_ops.cu).
 //
-// Every value is read once and written once, and the bound should be that; but a value comes with a dozen instructions, so the instructions
-// are what had to go: with a thread for eight neighbours, partners exchanged by shuffles and addresses formed for every head of every token 6534 tokens of 28
-// heads of 256 took 61-79 us.  Now a head is spread over head_dim / 8 lanes; a lane of the part that turns holds four elements and their partners
-// i + rot_dim / 2, and goes through four tokens with the same head: 46 us, 0.62 of the copy rate.  One token of one sequence takes 2.6 us from a graph, 5.4
-// called, which is the host's.  A norm is a reduction over the head's lanes.  The angles are the same for all heads of a token and computed once, in
-// shared memory, while the loads are under way.
+// Every value is read once and written once, and the bound should be that.  With a thread for eight neighbours, partners exchanged by shuffles and addresses
+// formed for every head of every token 6534 tokens of 28 heads of 256 took 61-79 us.  Now a head is spread over head_dim / 8 lanes; a lane of the part that
+// turns holds four elements and their partners i + rot_dim / 2, and goes through four tokens with the same head: 46 us, 0.62 of the copy rate, with 67 % of
+// the issue slots used and DRAM at 36 %: neither is the bound, but a block begins with its chain of look-ups and a barrier, and 1634 blocks, four an SM, are 2.8
+// rounds of them.  One token of one sequence takes 2.6 us from a graph, 5.5 to 6.5 called, which is the host's.  A norm is a reduction over the head's
+// lanes.  The angles are the same for all heads of a token and computed once, in shared memory, while the loads are under way.
 // position * inv_freq is formed and reduced to [-pi, pi] in FP64 (a float of 2^17 has steps of 1/64: the angle itself would be lost),
 // the reduced angle is rounded to FP32 (1.2e-7) for sincosf.
 #include <cuda_bf16.h>

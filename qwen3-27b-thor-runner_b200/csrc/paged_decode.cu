@@ -21,9 +21,9 @@
 //    nearly every rescaling of the results.
 //  * At an item's end the warps' results are added in shared memory in warp order.  Parts of a split item go to the handle's scratch and are added
 //    in block order by a second kernel.
-// Measured: 64 sequences of 128 to 16384 tokens, 24 heads over 2 of 256, 84 us, 0.77 of the copy rate in cache bytes; 243 sequences, 32 heads over 8 of 128,
-// 108 us, 0.79; one sequence of 131,000 tokens 56 us,
-// 0.74; one of 1501 16 us, a chain of latencies (lengths, pages, a few units, the sums, the join) and not bytes.
+// Measured, call after call (1.86 to 1.92 GHz under the power cap): 64 sequences of 128 to 16384 tokens, 24 heads over 2 of 256, 86 us, 0.75 of the copy rate in
+// cache bytes; 243 sequences, 32 heads over 8 of 128, 113 us, 0.76, and of 64 102 us; one sequence of 131,000 tokens 55 us, 0.74; one of 1501 16 us, a chain of
+// latencies (lengths, pages, a few units, the sums, the join) and not bytes.
 // Tokens past the length, and those of pages out of bounds, are zero-filled and masked, whatever memory holds there.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -624,7 +624,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_consta
 
 // Adds the parts of split items in the order of their blocks.  A kernel of its own behind the other one: there the last block to arrive would
 // read up to a hundred parts of 16 KB through one SM (17 us for a single long sequence, in two levels).  Here an item's 8-column tiles are spread over
-// blocks.  Few parts: a warp for each tile, all its parts under way at once.  Many: a block for one or two tiles, its warps share the parts.
+// blocks.  Few parts: a warp for each tile, all its parts under way at once.  Many: a block for one or two tiles, its warps share the parts.  (Heads of 256 spill 24
+// bytes at the 128 registers that two blocks an SM leave.)
 constexpr int kJoinWarps = 8, kJoinAhead = 10;
 template <int D>
 __global__ void __launch_bounds__(kJoinWarps * 32, 2)

@@ -153,8 +153,9 @@ NVFP4_PAGED_HD int part_slot(int first, int block) { return 2 * block + (block =
 constexpr int kLongChunk = 128;
 NVFP4_PAGED_HD int long_cost(int head_dim) { return head_dim == 256 ? 6 : 4; }
 
-// sum of floor((a i + b) / m) over 0 <= i < n (m > 0, a (n - 1) + b and a mod m * n + b mod m below 2^32), by swapping slope and modulus as in
-// Euclid's algorithm
+// sum of floor((a i + b) / m) over 0 <= i < n (m > 0, a (n - 1) + b and a mod m * n + b mod m below 2^32).  The published method for such sums: whole parts
+// of slope and offset are summed at once, and the points below the line that is left are counted along the other axis, which swaps slope and modulus as in Euclid's
+// algorithm (the reciprocity of floor sums, as in Graham, Knuth, Patashnik, Concrete Mathematics, 3.5)
 NVFP4_PAGED_HD long long floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
     long long sum = 0;
     while (n > 0) {

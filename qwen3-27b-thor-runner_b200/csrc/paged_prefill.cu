@@ -22,10 +22,14 @@
 // them, cut into equal runs, one persistent pair of blocks per pair of SMs; parts of split items (FP32 results, maxima, sums) are added by a second kernel.
 // Keys behind the item's last one and those of pages out of bounds are masked, and their values zeroed in shared memory, whatever lies there.
 //
-// Measured: a chunk of 256 tokens behind 16384 (24 heads over 2 of 256) 99 us, 1.05 PFLOP/s; a prompt of 8192 705-800 us by the clock the power leaves, 1.03 to
-// 1.17; 149 tokens 18 us, of which the products are 1.  A unit takes 2600 clocks with heads of 256 (products 2 x 1024, but the first one waits for shared memory,
-// 1500, and the second for tensor memory's operand, 1490; the weights 1900, over two buffers), 4200 for four tiles of 128; an item several thousand for
-// its way out (results from tensor memory, gates, rows written), which only the next item's loads and first scores overlap.
+// Measured, call after call under the power cap: a chunk of 256 tokens behind 16384 (24 heads over 2 of 256) 112-115 us at 1.7 GHz, 0.90 to 0.93 PFLOP/s; a prompt
+// of 8192 815-841 us at 1.6 GHz, 0.98 to 1.01 PFLOP/s (747 us in the first calls behind a pause); 149 tokens 18 us, of which the products are 1; a prompt
+// of 4096, 32 heads over 8 of 128, 175 us, 0.79 PFLOP/s, and of 64 148 us, 0.47.  A unit takes 2600 clocks with heads of 256 (products 2 x 1024, but the first one
+// waits for shared memory, 1500, and the second for tensor memory's operand, 1490; the weights 1900, over two buffers), 4200 for four tiles of 128; an item
+// several thousand for its way out (results from tensor memory, gates, rows written), which only the next item's loads and first scores overlap.
+//
+// The weights are rounded to BF16 for the second product, off by up to 2^-8 of each, which is the result's own rounding once more: 0.0018 to 0.0023 of the
+// result's norm against 64 bits, where one rounding has 0.0017.  A second operand with the remainders, as with few tokens, would be half as many products again.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -179,10 +183,6 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,"
         "%28,%29,%30,%31,%32};" ::"r"(taddr), NVFP4_S8(r, 0), NVFP4_S8(r, 8), NVFP4_S8(r, 16), NVFP4_S8(r, 24)
         : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), NVFP4_S8(r, 0), NVFP4_S8(r, 8)
-                 : "memory");
 }
 // What a load delivers is read behind the wait only: the registers pass through it.
 __device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
